@@ -270,6 +270,54 @@ int otx_rope_heads_bwd(const void* dy, const float* cos, const float* sin, void*
  * their backward. */
 int otx_swap_heads(const void* x, void* y, int B, int X, int Y, int D, int dtype, void* stream);
 
+/* Masked attention: document and prefix masks, padding, windows of any size,
+ * tanh-capped scores, a linear distance bias, any sequence length up to 2^24.
+ *   t_ij = softcap tanh(q_i.k_j / sqrt(D) / softcap)   (softcap 0: q_i.k_j / sqrt(D))
+ *   u_ij = t_ij - slopes[h] |i - j|                     (slopes NULL: t_ij)
+ *   o_i  = sum_j softmax(u_i)_j v_j over the visible j; a row that sees nothing is 0
+ *   j is visible to i when doc_ids[b][i] == doc_ids[b][j] >= 0 (doc_ids NULL: always) and
+ *   (j <= i and (window == 0 or i - j < window)) or j < prefix[b] (prefix NULL: 0)
+ * A negative document marks padding.  What lies in rows that a query does not
+ * see (NaN, infinities) does not reach it, in either direction.
+ * strides: of dimensions b, h and s in elements, for q, k, v, o (forward, 12
+ * values) and q, k, v, o, dout, dq, dk, dv (backward, 24); the last dimension is
+ * contiguous, rows start at 16-byte boundaries.  slopes float32 [H], doc_ids
+ * int32 [B, S], prefix int32 [B].  table: otx_mask_attn_table_bytes(B, S), written
+ * by the forward where doc_ids are given and read by the backward.  lse
+ * float32 [B, H, S], as the forward leaves it (units of log 2).
+ * These operators are not under the contract above: products run on the bf16
+ * matrix units with P and dS rounded to bf16 (binary32 tensors: on the binary32
+ * ones), sums and softmax statistics are binary32.  Results repeat bit for bit. */
+size_t otx_mask_attn_table_bytes(int B, int S);
+size_t otx_mask_attn_bwd_workspace_bytes(int B, int H, int Hkv, int S, int D);
+int otx_mask_attn_fwd(const void* q, const void* k, const void* v, void* o, float* lse, const float* slopes,
+                      const int32_t* doc_ids, const int32_t* prefix, void* table, const long* strides, int B, int H,
+                      int Hkv, int S, int D, int window, float softcap, int dtype, void* stream);
+int otx_mask_attn_bwd(const void* q, const void* k, const void* v, const void* o, const float* lse, const void* dout,
+                      void* dq, void* dk, void* dv, const float* slopes, const int32_t* doc_ids, const int32_t* prefix,
+                      const void* table, const long* strides, int B, int H, int Hkv, int S, int D, int window,
+                      float softcap, int dtype, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Rotary positions: columns 0 .. R - 1 of every head are turned in pairs, (2 i,
+ * 2 i + 1) in layout 0 and (i, i + R / 2) in layout 1, by the angle of the row's
+ * position (cos, sin float32 [P, R / 2]); the other columns are copied.
+ * positions int32 [B, T], or NULL: row t is position t.  A position outside
+ * 0 .. P - 1 turns its row to NaN.  backward: the transposed turn.  strides: of
+ * b, t and h in elements, for x and y; the last dimension is contiguous. */
+int otx_rotary(const void* x, const float* cos, const float* sin, const int32_t* positions, void* y,
+               const long* strides, int B, int T, int H, int D, int R, int P, int layout, int backward, int dtype,
+               void* stream);
+
+/* Layer norm of rows of D: y = (x - mean) rstd w + b (b NULL: 0); mean and rstd
+ * float32 [rows].  The backward writes dx and, in wdtype, dw and db (db NULL: not
+ * formed); sums in binary32 in a fixed order. */
+int otx_layer_norm_fwd(const void* x, const void* w, const void* b, void* y, float* mean, float* rstd, long rows, int D,
+                       float eps, int dtype, void* stream);
+size_t otx_layer_norm_bwd_workspace_bytes(long rows, int D);
+int otx_layer_norm_bwd(const void* x, const void* w, const float* mean, const float* rstd, const void* dy, void* dx,
+                       void* dw, void* db, long rows, int D, int dtype, int wdtype, void* workspace,
+                       size_t workspace_bytes, void* stream);
+
 /* Softmax scale used by the kernels: RN_binary32(1 / sqrt(D)). */
 float otx_softmax_scale(int D);
 

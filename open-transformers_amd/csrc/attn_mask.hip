@@ -1,0 +1,848 @@
+// Masked flash attention: document and prefix masks, padding, windows of any size, tanh-capped
+// scores and a linear distance bias, forward and backward, for any sequence length.
+//
+//   t_ij = cap tanh(sigma q_i.k_j / cap)  (or sigma q_i.k_j)      sigma = 1 / sqrt(D)
+//   u_ij = t_ij - slope_h |i - j|
+//   O_i  = sum_j p_ij v_j,  p_i = softmax of u_i over the visible j; a row that sees nothing is 0
+//   visible(i, j): doc_i == doc_j >= 0 and ((j <= i and (window == 0 or i - j < window)) or j < prefix_b)
+//
+//   D_i = dO_i.O_i   dU = P (dO V^T - D)   dS = dU (1 - (t / cap)^2)
+//   dQ = sigma dS K   dK = sigma dS^T Q   dV = P^T dO
+//
+// One pass over the keys with a running maximum and sum, all statistics and accumulators in
+// binary32.  The products run on the matrix units in the storage type: v_mfma_f32_32x32x16_bf16,
+// or v_mfma_f32_32x32x2_f32 for binary32 tensors.  P and dS are rounded to bf16 where they are
+// the operand of a bf16 product (half a step, 2^-9 relative, unbiased; the accumulation is
+// binary32).  No atomics: dQ and dK/dV are separate kernels that each own their output rows and
+// form S and dP themselves, so results repeat bit for bit.
+//
+// Layout.  A wave owns 32 rows (queries, or keys in the dK/dV kernel) and holds them as the
+// matrix unit's B operand; the other side's tile lies in LDS.  S^T = K Q^T then leaves every
+// lane with one query (lane % 32) and 16 keys of each 32-key block, so the softmax needs one
+// exchange between half-waves, and the result registers are, as they are, the B operand of the
+// next product O^T = V^T P^T: the k index of a product may be permuted when both operands are,
+// and the A operand is read from LDS with the same permutation (transposing reads,
+// ds_read_b64_tr_b16, for bf16).  P and dS never pass through LDS.
+//
+// Masked pairs contribute nothing, whatever their rows hold.  A weight of 0 times a NaN or an
+// infinity is NaN, so a tile that some rows of the workgroup do not see whole is checked for
+// non-finite values as it is staged, and such a tile takes a slow path that skips zero weights.
+#include "otx_args.h"
+#include "otx_common.h"
+
+namespace otx {
+
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef uint16_t u16x4 __attribute__((ext_vector_type(4)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef short s16x8 __attribute__((ext_vector_type(8)));
+
+namespace {
+
+constexpr float kLog2e = 1.44269504088896340736f;
+constexpr int kTab = 64;  // tokens per entry of the block table
+constexpr int kThreads = 256;
+
+// ---- matrix products of a storage type -----------------------------------------------------
+// Rows of a tile lie in LDS with D * sizeof(T) bytes each, cut into 16-byte chunks; chunk c of
+// row r is kept at position c ^ swizzle(r).
+template <typename T, int D>
+struct Tile {
+  static constexpr int NC = D * (int)sizeof(T) / 16;  // chunks in a row
+  static constexpr int KS = NC / 2;                   // steps over D of a row product (a chunk for each half-wave)
+  static constexpr int DT = D / 32;
+  static constexpr int RB = D * (int)sizeof(T);
+
+  static constexpr int SW = NC == 16 ? 15 : 7;
+  __device__ static __forceinline__ int swizzle(int row) { return row & SW; }
+  __device__ static __forceinline__ int at(int row, int chunk) { return row * RB + ((chunk ^ swizzle(row)) << 4); }
+  __device__ static __forceinline__ u32x4 row_frag(const char* lds, int row, int chunk) {
+    return *(const u32x4*)(lds + at(row, chunk));
+  }
+};
+
+template <typename T>
+__device__ __forceinline__ f32x16 mma_rows(u32x4 a, u32x4 b, f32x16 c) {
+  if constexpr (sizeof(T) == 2) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0,
+                                                   0);
+  } else {
+    c = __builtin_amdgcn_mfma_f32_32x32x2f32(otx_u2f(a.x), otx_u2f(b.x), c, 0, 0, 0);
+    c = __builtin_amdgcn_mfma_f32_32x32x2f32(otx_u2f(a.y), otx_u2f(b.y), c, 0, 0, 0);
+    c = __builtin_amdgcn_mfma_f32_32x32x2f32(otx_u2f(a.z), otx_u2f(b.z), c, 0, 0, 0);
+    return __builtin_amdgcn_mfma_f32_32x32x2f32(otx_u2f(a.w), otx_u2f(b.w), c, 0, 0, 0);
+  }
+}
+
+// acc[dt][d][n] += sum over the 32 tile rows k0 + 0..31 of X[k][32 dt + d] W[k][n], W in result layout.
+template <typename T, int D>
+__device__ __forceinline__ void mma_cols(f32x16 (&acc)[D / 32], const char* lds, int k0, const f32x16& w, int lane) {
+  using L = Tile<T, D>;
+  const int h = lane >> 5;
+  if constexpr (sizeof(T) == 2) {
+#pragma unroll
+    for (int s = 0; s < 2; s++) {
+      bf16x8 b;
+#pragma unroll
+      for (int j = 0; j < 8; j++) b[j] = (__bf16)w[8 * s + j];
+      // 16 lanes of a transposing read take rows k .. k + 3, columns 16 g .. 16 g + 15: lane i
+      // addresses row k + i / 4, columns 4 (i % 4) .., and receives column i of the four rows
+      const int row = k0 + 16 * s + 4 * h + ((lane & 15) >> 2);
+      const int col = 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+#pragma unroll
+      for (int dt = 0; dt < L::DT; dt++) {
+        const int c = (32 * dt + col) >> 3, off = (col & 7) * 2;
+        typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+        const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(lds + L::at(row, c) + off));
+        const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(lds + L::at(row + 8, c) + off));
+        const s16x8 a = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+        acc[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), b, acc[dt], 0, 0, 0);
+      }
+    }
+  } else {
+#pragma unroll
+    for (int r = 0; r < 16; r++) {
+      const int row = k0 + otx_row(r, 0) + 4 * h;
+#pragma unroll
+      for (int dt = 0; dt < L::DT; dt++) {
+        const int c = 8 * dt + ((lane & 31) >> 2);
+        const float a = *(const float*)(lds + L::at(row, c) + (lane & 3) * 4);
+        acc[dt] = __builtin_amdgcn_mfma_f32_32x32x2f32(a, w[r], acc[dt], 0, 0, 0);
+      }
+    }
+  }
+}
+
+// mma_cols for a tile with non-finite values: a row of zero weight is left out.
+template <typename T, int D>
+__device__ __forceinline__ void cols_skipping(f32x16 (&acc)[D / 32], const char* lds, int k0, f32x16 w, int lane) {
+  using L = Tile<T, D>;
+  constexpr int E = 16 / (int)sizeof(T);
+#pragma unroll 1
+  for (int r = 0; r < 16; r++) {
+    const float mine = w[0];
+#pragma unroll
+    for (int i = 0; i < 15; i++) w[i] = w[i + 1];
+#pragma unroll 1
+    for (int from = 0; from < 2; from++) {
+      const float x = __shfl(mine, (lane & 31) + 32 * from);
+      int row = k0 + 8 * (r >> 2) + 4 * from + (r & 3), d0 = 4 * (lane >> 5);
+      asm("" : "+v"(row), "+v"(d0));  // addresses are formed here, not kept in registers across the kernel
+#pragma unroll
+      for (int dt = 0; dt < L::DT; dt++)
+#pragma unroll
+        for (int g = 0; g < 4; g++) {
+          const int d = 32 * dt + 8 * g + d0;
+          const T* p = (const T*)(lds + L::at(row, d / E)) + d % E;
+#pragma unroll
+          for (int i = 0; i < 4; i++) {
+            const float y = __builtin_fmaf(x, Elem<T>::ld(p + i), acc[dt][4 * g + i]);
+            acc[dt][4 * g + i] = x != 0.0f ? y : acc[dt][4 * g + i];
+          }
+        }
+    }
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ float element(const u32x4& v, int e) {
+  if constexpr (sizeof(T) == 4) return otx_u2f(v[e]);
+  return otx_u2f((e & 1) ? (v[e >> 1] & 0xffff0000u) : (v[e >> 1] << 16));
+}
+
+// Whether a 16-byte chunk holds an infinity or a NaN.
+template <typename T>
+__device__ __forceinline__ bool nonfinite(const u32x4& v) {
+  bool bad = false;
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    const uint32_t x = v[i];
+    bad |= (x & 0x7f800000u) == 0x7f800000u;
+    if constexpr (sizeof(T) == 2) bad |= (x & 0x7f80u) == 0x7f80u;
+  }
+  return bad;
+}
+
+// ---- which tiles take part -------------------------------------------------------------------
+struct Band {  // the mask of one batch row, apart from documents
+  int S, window, prefix;
+  __device__ __forceinline__ bool any(int q0, int q1, int k0, int k1) const {  // some pair of the rectangle
+    return (k0 <= q1 && (window == 0 || k1 > q0 - window)) || k0 < prefix;
+  }
+  __device__ __forceinline__ bool all(int q0, int q1, int k0, int k1) const {  // every pair
+    return (k1 <= q0 && (window == 0 || k0 > q1 - window)) || k1 < prefix;
+  }
+};
+
+struct Docs {  // documents of a range of tokens
+  int lo, hi, pad;
+};
+__device__ __forceinline__ Docs docs_of(const i32x4* table, int first, int last, int nb) {
+  if (!table) return {0, 0, 0};
+  Docs d = {0x7fffffff, -1, 0};
+  for (int i = first; i <= last && i < nb; i++) {
+    const i32x4 t = table[i];
+    d.lo = min(d.lo, t.x);
+    d.hi = max(d.hi, t.y);
+    d.pad |= t.z;
+  }
+  return d;
+}
+
+// The tiles of BT tokens that a range of `own` tokens meets, ascending.  Lanes test 64 tiles at a time.
+template <int BT, bool OWN_QUERIES>
+struct TileIter {
+  uint64_t act, whole;  // whole: one document, no padding, no token past the end
+  int base, n, current;
+  Docs own;
+  int o0, o1;
+  __device__ __forceinline__ void init(int own0, int own1, const Docs& d, int ntiles) {
+    o0 = own0, o1 = own1, own = d, n = ntiles, act = 0, base = -64;
+  }
+  // The next tile, or -1; `same` says whether documents and the end leave it whole.
+  __device__ __forceinline__ int next(const Band& band, const i32x4* table, int nb, int lane, bool* same) {
+    while (act == 0) {
+      base += 64;
+      if (base >= n) return -1;
+      const int t = base + lane, t0 = t * BT, t1 = t0 + BT - 1;
+      bool a = false, w = false;
+      if (t < n) {
+        a = OWN_QUERIES ? band.any(o0, o1, t0, t1) : band.any(t0, t1, o0, o1);
+        w = t1 < band.S;
+        if (a && table) {
+          const Docs d = docs_of(table, t0 / kTab, t1 / kTab, nb);
+          a = d.lo <= own.hi && own.lo <= d.hi;
+          w = w && d.lo == d.hi && own.lo == own.hi && !d.pad && !own.pad;
+        }
+      }
+      act = __ballot(a);
+      whole = __ballot(w);
+    }
+    const int i = __builtin_ctzll(act);
+    act &= act - 1;
+    *same = (whole >> i) & 1;
+    return base + i;
+  }
+};
+
+// Which of the pairs of one owned row and 32 rows of a tile take part: bit r for element r of a
+// result block.  The owned row is query i against keys o0 + otx_row(r, h), or key i against queries.
+template <bool OWN_QUERIES>
+__device__ __forceinline__ uint32_t visible(const Band& band, const int* lid, int o, int own, int id, int h) {
+  // relative to the first tile row of this half-wave: lo < row <= hi, or (queries own) row < pre
+  const int base = o + 4 * h, w = band.window ? band.window : 0x40000000;
+  const int hi = OWN_QUERIES ? own - base : own + w - 1 - base;
+  const int lo = OWN_QUERIES ? own - w - base : own - 1 - base;
+  const int pre = OWN_QUERIES ? band.prefix - base : own < band.prefix ? 0x40000000 : -0x40000000;
+  uint32_t bits = 0;
+#pragma unroll
+  for (int g = 0; g < 4; g++) {
+    const i32x4 ids = *(const i32x4*)(lid + 8 * g + 4 * h);
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      const int row = 8 * g + i;
+      const bool see = (((row <= hi) & (row > lo)) | (row < pre)) & (ids[i] == id);
+      bits |= see ? 1u << (4 * g + i) : 0u;
+    }
+  }
+  return bits;
+}
+
+// x, as a value the compiler does not know to be the same in every tile: LDS addresses formed from it
+// are computed where they are used, and do not occupy registers across the kernel.
+__device__ __forceinline__ int opaque(int x) {
+  asm volatile("" : "+v"(x));
+  return x;
+}
+
+// The identity that pairs are matched by: the document, or a value that matches nothing.
+__device__ __forceinline__ int match_id(const int* doc, int i, int S, int none) {
+  if (i >= S) return none;
+  const int d = doc ? doc[i] : 0;
+  return d < 0 ? none : d;
+}
+
+__device__ __forceinline__ float swap_halves(float x) { return __shfl_xor(x, 32); }
+
+// tanh-capped score in units of log 2, from a raw dot product; for the backward t / cap is kept.
+template <typename T>
+__device__ __forceinline__ float cap_tanh(float s, float sigma_over_cap) {
+  if constexpr (sizeof(T) == 4) {
+    return tanhf(s * sigma_over_cap);
+  } else {  // 1 - 2 / (e^2x + 1): absolute error of a few 2^-24, far below a bf16 score's own
+    const float e = __builtin_amdgcn_exp2f(s * (2.0f * kLog2e * sigma_over_cap));
+    return __builtin_fmaf(-2.0f, __builtin_amdgcn_rcpf(e + 1.0f), 1.0f);
+  }
+}
+
+// ---- staging -------------------------------------------------------------------------------------
+// BT rows of a tensor, copied straight into LDS (16 bytes a lane, no registers); rows past the end
+// repeat the last one.  A wave's copy fills consecutive LDS, so the swizzle is applied to the chunk
+// that a lane fetches.
+template <typename T, int D, int BT>
+struct Stage {
+  using L = Tile<T, D>;
+  static constexpr int N = BT * L::NC / kThreads, RS = kThreads / L::NC;  // steps, rows a step
+  static_assert(BT * L::NC % kThreads == 0 && RS % (L::SW + 1) == 0, "a step keeps the swizzle");
+  const char* base;
+  int stride, off;  // bytes
+  __device__ __forceinline__ void init(const T* p, long s) {
+    const int r = threadIdx.x / L::NC, c = (threadIdx.x % L::NC) ^ L::swizzle(r);
+    base = (const char*)p, stride = (int)s * (int)sizeof(T), off = r * stride + c * 16;
+  }
+  __device__ __forceinline__ void copy(char* lds, int row0, int S) const {
+    const char* p = base + (long)row0 * stride;
+    char* to = lds + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) * 1024;
+    const int last = S - 1 - row0;
+    if (last >= BT - 1) {
+#pragma unroll
+      for (int i = 0; i < N; i++) otx_dma16(p + (long)i * RS * stride + off, to + i * kThreads * 16);
+    } else {
+      const int r = threadIdx.x / L::NC;
+#pragma unroll
+      for (int i = 0; i < N; i++)
+        otx_dma16(p + (off + (min(r + i * RS, last) - r) * stride), to + i * kThreads * 16);
+    }
+  }
+  // Whether this thread's share of a tile in LDS holds an infinity or a NaN.
+  __device__ __forceinline__ static bool bad(const char* lds) {
+    bool b = false;
+#pragma unroll
+    for (int i = 0; i < N; i++) b |= nonfinite<T>(*(const u32x4*)(lds + (threadIdx.x + i * kThreads) * 16));
+    return b;
+  }
+};
+
+// This wave's copies have arrived; with the barrier after it, everybody's.
+__device__ __forceinline__ void arrived() {
+  __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
+  __syncthreads();
+}
+
+template <typename T, int D>
+__device__ __forceinline__ void load_own(u32x4 (&f)[D * sizeof(T) / 32], const T* base, long stride, int row, int lane) {
+#pragma unroll
+  for (int ks = 0; ks < Tile<T, D>::KS; ks++)
+    f[ks] = *(const u32x4*)(base + (long)row * stride + (2 * ks + (lane >> 5)) * (16 / (int)sizeof(T)));
+}
+
+// Writes acc^T (column n = this lane's row) times f into a row of an output tensor.
+template <typename T, int D>
+__device__ __forceinline__ void store_own(T* row, const f32x16 (&acc)[D / 32], float f, int lane) {
+#pragma unroll
+  for (int dt = 0; dt < D / 32; dt++)
+#pragma unroll
+    for (int g = 0; g < 4; g++) {
+      T* p = row + 32 * dt + 8 * g + 4 * (lane >> 5);
+      if constexpr (sizeof(T) == 2) {
+        u16x4 o;
+        o.x = Elem<T>::put(acc[dt][4 * g] * f), o.y = Elem<T>::put(acc[dt][4 * g + 1] * f);
+        o.z = Elem<T>::put(acc[dt][4 * g + 2] * f), o.w = Elem<T>::put(acc[dt][4 * g + 3] * f);
+        *(u16x4*)p = o;
+      } else {
+        *(float4*)p = make_float4(acc[dt][4 * g] * f, acc[dt][4 * g + 1] * f, acc[dt][4 * g + 2] * f,
+                                  acc[dt][4 * g + 3] * f);
+      }
+    }
+}
+
+// The head that the i-th of n = B * H work items of a row of the grid takes.  Workgroups go round
+// the 8 XCDs; where n allows, each XCD gets a run of neighbouring heads, whose keys its L2 then holds.
+__device__ __forceinline__ int spread(int i, int n) { return n % 8 == 0 ? (i % 8) * (n / 8) + i / 8 : i; }
+
+template <typename T> constexpr int tile_rows() { return sizeof(T) == 2 ? 64 : 32; }
+
+// ---- block table ---------------------------------------------------------------------------------
+__global__ void __launch_bounds__(256) mask_table_kernel(const int* doc, i32x4* table, int B, int S, int nb) {
+  const int lane = threadIdx.x & 63;
+  const long n = (long)B * nb;
+  for (long w = (long)blockIdx.x * 4 + (threadIdx.x >> 6); w < n; w += (long)gridDim.x * 4) {
+    const long b = w / nb;
+    const int i = (int)(w % nb) * kTab + lane;
+    const int d = i < S ? doc[b * S + i] : 0;
+    int lo = i < S && d >= 0 ? d : 0x7fffffff, hi = i < S && d >= 0 ? d : -1;
+    for (int m = 32; m; m >>= 1) {
+      lo = min(lo, __shfl_xor(lo, m));
+      hi = max(hi, __shfl_xor(hi, m));
+    }
+    const int pad = __ballot(i < S && d < 0) != 0;
+    if (lane == 0) table[w] = i32x4{lo, hi, pad, 0};
+  }
+}
+
+// ---- forward -------------------------------------------------------------------------------------
+// Tiles are copied one ahead into the other of two buffers, with one barrier a tile.
+template <typename T, int D, bool PLAIN>
+__global__ void __launch_bounds__(kThreads, 2) mask_attn_fwd_kernel(const MaskAttnArgs a) {
+  using L = Tile<T, D>;
+  constexpr int BN = tile_rows<T>(), NT = BN / 32, BM = 128, BYTES = BN * L::RB;
+  __shared__ __align__(1024) char lk0[BYTES], lv0[BYTES], lk1[BYTES], lv1[BYTES];
+  __shared__ __align__(16) int lid[BN];
+  __shared__ int lbad;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5;
+  const int S = a.S, nq = (S + BM - 1) / BM, nk = (S + BN - 1) / BN, nb = (S + kTab - 1) / kTab;
+  const long total = (long)a.B * a.H * nq;
+  const float cs = a.sigma * kLog2e;
+  if (threadIdx.x == 0) lbad = -1;
+  int seq = 0;  // tiles so far: lbad names the last one that held a non-finite value
+
+  for (long w = blockIdx.x; w < total; w += gridDim.x) {
+    const int bh = spread((int)(w % (a.B * a.H)), a.B * a.H), b = bh / a.H, hq = bh % a.H, hk = hq / (a.H / a.Hkv);
+    const int q0 = (nq - 1 - (int)(w / (a.B * a.H))) * BM, q1 = min(q0 + BM, S) - 1;
+    const int qw0 = q0 + 32 * wave, qw1 = min(qw0 + 31, S - 1), qi = qw0 + (lane & 31);
+    const int* doc = a.doc ? a.doc + (long)b * S : nullptr;
+    const i32x4* table = a.doc ? (const i32x4*)a.table + (long)b * nb : nullptr;
+    const Band band = {S, a.window, a.prefix ? min(max(a.prefix[b], 0), S) : 0};
+    const float slope = !PLAIN && a.slopes ? a.slopes[hq] * kLog2e : 0.0f;
+    Stage<T, D, BN> gk, gv;
+    gk.init((const T*)a.k + b * a.sk[0] + hk * a.sk[1], a.sk[2]);
+    gv.init((const T*)a.v + b * a.sv[0] + hk * a.sv[1], a.sv[2]);
+
+    TileIter<BN, true> it;
+    it.init(q0, q1, docs_of(table, q0 / kTab, q1 / kTab, nb), nk);
+    bool same = false;
+    int kb = it.next(band, table, nb, lane, &same);
+    __syncthreads();  // the last item's tiles have been read
+    if (kb >= 0) {
+      gk.copy(lk0, kb * BN, S);
+      gv.copy(lv0, kb * BN, S);
+    }
+    u32x4 qf[L::KS];
+    load_own<T, D>(qf, (const T*)a.q + b * a.sq[0] + hq * a.sq[1], a.sq[2], min(qi, S - 1), lane);
+    const int qid = match_id(doc, qi, S, -2);
+    f32x16 acc[L::DT] = {};
+    float m = -INFINITY, l = 0.0f;
+
+    auto tile = [&](const char* lk, const char* lv, char* nlk, char* nlv) {
+      const int lane = opaque(threadIdx.x & 63), h = lane >> 5;
+      const int k0 = kb * BN, k1 = k0 + BN - 1;
+      const bool cut = !same || !band.all(q0, q1, k0, k1);  // some row of the workgroup does not see it whole
+      const bool masked = !same || !band.all(qw0, qw1, k0, k1);
+      arrived();
+      kb = it.next(band, table, nb, lane, &same);
+      if (kb >= 0) {
+        gk.copy(nlk, kb * BN, S);
+        gv.copy(nlv, kb * BN, S);
+      }
+      bool bad = false;
+      if (cut) {
+        if (threadIdx.x < BN) lid[threadIdx.x] = match_id(doc, k0 + threadIdx.x, S, -1);
+        if (gv.bad(lv)) lbad = seq;
+        __syncthreads();
+        bad = lbad == seq;
+      }
+      seq++;
+      if (!band.any(qw0, qw1, k0, k1)) return;
+      f32x16 s[NT] = {};
+#pragma unroll
+      for (int t = 0; t < NT; t++)
+#pragma unroll
+        for (int ks = 0; ks < L::KS; ks++)
+          s[t] = mma_rows<T>(L::row_frag(lk, 32 * t + (lane & 31), 2 * ks + h), qf[ks], s[t]);
+      if constexpr (!PLAIN) {  // to scores in units of log 2
+        if (a.cap > 0.0f) {
+          const float soc = a.sigma / a.cap, cl = a.cap * kLog2e;
+#pragma unroll
+          for (int t = 0; t < NT; t++)
+#pragma unroll
+            for (int r = 0; r < 16; r++) s[t][r] = cl * cap_tanh<T>(s[t][r], soc);
+        } else {
+#pragma unroll
+          for (int t = 0; t < NT; t++)
+#pragma unroll
+            for (int r = 0; r < 16; r++) s[t][r] *= cs;
+        }
+        if (a.slopes) {
+#pragma unroll
+          for (int t = 0; t < NT; t++)
+#pragma unroll
+            for (int r = 0; r < 16; r++)
+              s[t][r] = __builtin_fmaf(-slope, fabsf((float)(qi - (k0 + 32 * t + otx_row(r, 0) + 4 * h))), s[t][r]);
+        }
+      }
+      if (masked) {
+#pragma unroll
+        for (int t = 0; t < NT; t++) {
+          const uint32_t see = visible<true>(band, lid + 32 * t, k0 + 32 * t, qi, qid, h);
+#pragma unroll
+          for (int r = 0; r < 16; r++) s[t][r] = (see >> r) & 1 ? s[t][r] : -INFINITY;
+        }
+      }
+      float top = s[0][0];
+#pragma unroll
+      for (int t = 0; t < NT; t++)
+#pragma unroll
+        for (int r = 0; r < 16; r++) top = fmaxf(top, s[t][r]);
+      top = fmaxf(top, swap_halves(top));
+      if constexpr (PLAIN) top *= cs;
+      // The statistics move only where a maximum grows by more than 2^8: weights stay below 2^8 and
+      // the sums, in binary32, lose nothing; most tiles then leave the accumulator as it is.
+      if (__ballot(top > m + 8.0f)) {
+        const float mn = fmaxf(m, top), f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - mn);
+        m = mn;
+        l *= f;
+#pragma unroll
+        for (int dt = 0; dt < L::DT; dt++)
+#pragma unroll
+          for (int r = 0; r < 16; r++) acc[dt][r] *= f;
+      }
+      const float mu = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+      for (int t = 0; t < NT; t++) {
+#pragma unroll
+        for (int r = 0; r < 16; r++) {
+          s[t][r] = __builtin_amdgcn_exp2f(PLAIN ? __builtin_fmaf(s[t][r], cs, -mu) : s[t][r] - mu);
+          l += s[t][r];
+        }
+      }
+      if (bad) {
+#pragma unroll
+        for (int t = 0; t < NT; t++) cols_skipping<T, D>(acc, lv, 32 * t, s[t], lane);
+      } else {
+#pragma unroll
+        for (int t = 0; t < NT; t++) mma_cols<T, D>(acc, lv, 32 * t, s[t], lane);
+      }
+    };
+    while (kb >= 0) {
+      tile(lk0, lv0, lk1, lv1);
+      if (kb < 0) break;
+      tile(lk1, lv1, lk0, lv0);
+    }
+    l += swap_halves(l);
+    if (qi < S) {
+      store_own<T, D>((T*)a.out + b * a.so[0] + hq * a.so[1] + qi * a.so[2], acc, l == 0.0f ? 0.0f : 1.0f / l, lane);
+      if (h == 0) a.lse[((long)b * a.H + hq) * S + qi] = l == 0.0f ? 0.0f : m + __builtin_log2f(l);
+    }
+  }
+}
+
+// ---- backward: the weight and its gradient of one pair ------------------------------------------------
+// Element r of sv holds the raw dot product q.k, of dpv the product dO.v; on return p and dS (without sigma).
+template <typename T, bool PLAIN>
+__device__ __forceinline__ void weight(const MaskAttnArgs& a, f32x16& sv, f32x16& dpv, int r, float slope, float cs,
+                                       float lse, float dsum, int delta) {
+  const float s = sv[r], dp = dpv[r];
+  float u = s * cs, g = 1.0f;
+  if constexpr (PLAIN) {
+    sv[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s, cs, -lse));
+  } else {
+    if (a.cap > 0.0f) {
+      const float t = cap_tanh<T>(s, a.sigma / a.cap);
+      u = a.cap * kLog2e * t;
+      g = __builtin_fmaf(-t, t, 1.0f);
+    }
+    if (a.slopes) u = __builtin_fmaf(-slope, fabsf((float)delta), u);
+    sv[r] = __builtin_amdgcn_exp2f(u - lse);
+  }
+  dpv[r] = sv[r] * (dp - dsum) * g;
+}
+
+// ---- backward: dQ, and D_i on the way ---------------------------------------------------------------
+template <typename T, int D, bool PLAIN>
+__global__ void __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) mask_attn_dq_kernel(const MaskAttnArgs a) {
+  using L = Tile<T, D>;
+  constexpr int BN = tile_rows<T>(), NT = BN / 32, BM = 128, BYTES = BN * L::RB;
+  __shared__ __align__(1024) char lk0[BYTES], lv0[BYTES], lk1[BYTES], lv1[BYTES];
+  __shared__ __align__(16) int lid[BN];
+  __shared__ int lbad;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5;
+  const int S = a.S, nq = (S + BM - 1) / BM, nk = (S + BN - 1) / BN, nb = (S + kTab - 1) / kTab;
+  const long total = (long)a.B * a.H * nq;
+  const float cs = a.sigma * kLog2e;
+  if (threadIdx.x == 0) lbad = -1;
+  int seq = 0;
+
+  for (long w = blockIdx.x; w < total; w += gridDim.x) {
+    const int bh = spread((int)(w % (a.B * a.H)), a.B * a.H), b = bh / a.H, hq = bh % a.H, hk = hq / (a.H / a.Hkv);
+    const int q0 = (nq - 1 - (int)(w / (a.B * a.H))) * BM, q1 = min(q0 + BM, S) - 1;
+    const int qw0 = q0 + 32 * wave, qw1 = min(qw0 + 31, S - 1), qi = qw0 + (lane & 31), qr = min(qi, S - 1);
+    const int* doc = a.doc ? a.doc + (long)b * S : nullptr;
+    const i32x4* table = a.doc ? (const i32x4*)a.table + (long)b * nb : nullptr;
+    const Band band = {S, a.window, a.prefix ? min(max(a.prefix[b], 0), S) : 0};
+    const float slope = !PLAIN && a.slopes ? a.slopes[hq] * kLog2e : 0.0f;
+    Stage<T, D, BN> gk, gv;
+    gk.init((const T*)a.k + b * a.sk[0] + hk * a.sk[1], a.sk[2]);
+    gv.init((const T*)a.v + b * a.sv[0] + hk * a.sv[1], a.sv[2]);
+
+    TileIter<BN, true> it;
+    it.init(q0, q1, docs_of(table, q0 / kTab, q1 / kTab, nb), nk);
+    bool same = false;
+    int kb = it.next(band, table, nb, lane, &same);
+    __syncthreads();
+    if (kb >= 0) {
+      gk.copy(lk0, kb * BN, S);
+      gv.copy(lv0, kb * BN, S);
+    }
+    u32x4 qf[L::KS], gf[L::KS];
+    load_own<T, D>(qf, (const T*)a.q + b * a.sq[0] + hq * a.sq[1], a.sq[2], qr, lane);
+    load_own<T, D>(gf, (const T*)a.dout + b * a.sdo[0] + hq * a.sdo[1], a.sdo[2], qr, lane);
+    float dsum = 0.0f;
+    {
+      const T* op = (const T*)a.o + b * a.so[0] + hq * a.so[1] + qr * a.so[2];
+#pragma unroll
+      for (int ks = 0; ks < L::KS; ks++) {
+        const u32x4 of = *(const u32x4*)(op + (2 * ks + h) * (16 / (int)sizeof(T)));
+#pragma unroll
+        for (int e = 0; e < Elem<T>::VEC; e++)
+          dsum = __builtin_fmaf(element<T>(gf[ks], e), element<T>(of, e), dsum);
+      }
+      dsum += swap_halves(dsum);
+    }
+    const long row = ((long)b * a.H + hq) * S + qr;
+    if (qi < S && h == 0) a.dsum[row] = dsum;
+    const float lse = a.lse[row];
+    const int qid = match_id(doc, qi, S, -2);
+    f32x16 acc[L::DT] = {};
+
+    auto tile = [&](const char* lk, const char* lv, char* nlk, char* nlv) {
+      const int lane = opaque(threadIdx.x & 63), h = lane >> 5;
+      const int k0 = kb * BN, k1 = k0 + BN - 1;
+      const bool cut = !same || !band.all(q0, q1, k0, k1);
+      const bool masked = !same || !band.all(qw0, qw1, k0, k1);
+      arrived();
+      kb = it.next(band, table, nb, lane, &same);
+      if (kb >= 0) {
+        gk.copy(nlk, kb * BN, S);
+        gv.copy(nlv, kb * BN, S);
+      }
+      bool bad = false;
+      if (cut) {
+        if (threadIdx.x < BN) lid[threadIdx.x] = match_id(doc, k0 + threadIdx.x, S, -1);
+        if (gk.bad(lk)) lbad = seq;
+        __syncthreads();
+        bad = lbad == seq;
+      }
+      seq++;
+      if (!band.any(qw0, qw1, k0, k1)) return;
+#pragma unroll
+      for (int t = 0; t < NT; t++) {
+        f32x16 s = {}, dp = {};
+#pragma unroll
+        for (int ks = 0; ks < L::KS; ks++) {
+          s = mma_rows<T>(L::row_frag(lk, 32 * t + (lane & 31), 2 * ks + h), qf[ks], s);
+          dp = mma_rows<T>(L::row_frag(lv, 32 * t + (lane & 31), 2 * ks + h), gf[ks], dp);
+        }
+#pragma unroll
+        for (int r = 0; r < 16; r++)
+          weight<T, PLAIN>(a, s, dp, r, slope, cs, lse, dsum, qi - (k0 + 32 * t + 4 * h + otx_row(r, 0)));
+        if (masked) {
+          const uint32_t see = visible<true>(band, lid + 32 * t, k0 + 32 * t, qi, qid, h);
+#pragma unroll
+          for (int r = 0; r < 16; r++) dp[r] = (see >> r) & 1 ? dp[r] : 0.0f;
+        }
+        if (bad)
+          cols_skipping<T, D>(acc, lk, 32 * t, dp, lane);
+        else
+          mma_cols<T, D>(acc, lk, 32 * t, dp, lane);
+      }
+    };
+    while (kb >= 0) {
+      tile(lk0, lv0, lk1, lv1);
+      if (kb < 0) break;
+      tile(lk1, lv1, lk0, lv0);
+    }
+    if (qi < S) store_own<T, D>((T*)a.dq + b * a.sdq[0] + hq * a.sdq[1] + qi * a.sdq[2], acc, a.sigma, lane);
+  }
+}
+
+// ---- backward: dK and dV ----------------------------------------------------------------------------
+// SPLIT: a workgroup takes one query head and writes binary32 sums to a.part, which
+// mask_attn_join_kernel adds over the group; otherwise it takes the group's heads one after the other.
+template <typename T, int D, bool PLAIN, bool SPLIT>
+__global__ void __launch_bounds__(kThreads, sizeof(T) * D == 128 ? 2 : 1) mask_attn_dkdv_kernel(const MaskAttnArgs a) {
+  using L = Tile<T, D>;
+  constexpr int BN = tile_rows<T>(), NT = BN / 32, BM = 128, BYTES = BN * L::RB;  // BM keys owned, BN queries a tile
+  __shared__ __align__(1024) char lq0[BYTES], lg0[BYTES], lq1[BYTES], lg1[BYTES];
+  __shared__ __align__(16) float ll[2][64], ld[2][64];
+  __shared__ __align__(16) int lid[BN];
+  __shared__ int lbad;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5;
+  const int S = a.S, nkb = (S + BM - 1) / BM, nq = (S + BN - 1) / BN, nb = (S + kTab - 1) / kTab;
+  const int group = a.H / a.Hkv, heads = SPLIT ? a.H : a.Hkv;
+  const long total = (long)a.B * heads * nkb;
+  const float cs = a.sigma * kLog2e;
+  if (threadIdx.x == 0) lbad = -1;
+  int seq = 0;
+
+  for (long w = blockIdx.x; w < total; w += gridDim.x) {
+    const int bh = spread((int)(w % (a.B * heads)), a.B * heads), b = bh / heads;
+    const int hk = SPLIT ? bh % heads / group : bh % heads;
+    const int k0 = (int)(w / (a.B * heads)) * BM, k1 = min(k0 + BM, S) - 1;  // the first keys have the most queries
+    const int kw0 = k0 + 32 * wave, kw1 = min(kw0 + 31, S - 1), kj = kw0 + (lane & 31), kr = min(kj, S - 1);
+    const int* doc = a.doc ? a.doc + (long)b * S : nullptr;
+    const i32x4* table = a.doc ? (const i32x4*)a.table + (long)b * nb : nullptr;
+    const Band band = {S, a.window, a.prefix ? min(max(a.prefix[b], 0), S) : 0};
+    const Docs own = docs_of(table, k0 / kTab, k1 / kTab, nb);
+
+    u32x4 kf[L::KS], vf[L::KS];
+    load_own<T, D>(kf, (const T*)a.k + b * a.sk[0] + hk * a.sk[1], a.sk[2], kr, lane);
+    load_own<T, D>(vf, (const T*)a.v + b * a.sv[0] + hk * a.sv[1], a.sv[2], kr, lane);
+    const int kid = match_id(doc, kj, S, -1);
+    f32x16 dk[L::DT] = {}, dv[L::DT] = {};
+
+    const int first = SPLIT ? bh % heads : hk * group, last = SPLIT ? first + 1 : first + group;
+    for (int hq = first; hq < last; hq++) {
+      const long row0 = ((long)b * a.H + hq) * S;
+      const float slope = !PLAIN && a.slopes ? a.slopes[hq] * kLog2e : 0.0f;
+      Stage<T, D, BN> gq, gg;
+      gq.init((const T*)a.q + b * a.sq[0] + hq * a.sq[1], a.sq[2]);
+      gg.init((const T*)a.dout + b * a.sdo[0] + hq * a.sdo[1], a.sdo[2]);
+      TileIter<BN, false> it;
+      it.init(k0, k1, own, nq);
+      bool same = false;
+      int qb = it.next(band, table, nb, lane, &same);
+      auto stage = [&](char* lq, char* lg, int buf) {
+        gq.copy(lq, qb * BN, S);
+        gg.copy(lg, qb * BN, S);
+        const long i = row0 + min(qb * BN + lane, S - 1);  // 64 rows, BN of them read
+        if (wave == 0) otx_dma4(a.lse + i, ll[buf]);
+        if (wave == 1) otx_dma4(a.dsum + i, ld[buf]);
+      };
+      __syncthreads();
+      if (qb >= 0) stage(lq0, lg0, 0);
+
+      auto tile = [&](const char* lq, const char* lg, const int buf, char* nlq, char* nlg) {
+      const int lane = opaque(threadIdx.x & 63), h = lane >> 5;
+        const int q0 = qb * BN, q1 = q0 + BN - 1;
+        const bool cut = !same || k0 + BM > S || !band.all(q0, q1, k0, k0 + BM - 1);
+        const bool masked = !same || kw0 + 32 > S || !band.all(q0, q1, kw0, kw0 + 31);
+        arrived();
+        qb = it.next(band, table, nb, lane, &same);
+        if (qb >= 0) stage(nlq, nlg, 1 - buf);
+        bool bad = false;
+        if (cut) {
+          if (threadIdx.x < BN) lid[threadIdx.x] = match_id(doc, q0 + threadIdx.x, S, -2);
+          if (gq.bad(lq) || gg.bad(lg)) lbad = seq;
+          __syncthreads();
+          bad = lbad == seq;
+        }
+        seq++;
+        if (kw0 >= S || !band.any(q0, min(q1, S - 1), kw0, kw1)) return;
+#pragma unroll
+        for (int t = 0; t < NT; t++) {
+          f32x16 s = {}, dp = {};
+#pragma unroll
+          for (int ks = 0; ks < L::KS; ks++) {
+            s = mma_rows<T>(L::row_frag(lq, 32 * t + (lane & 31), 2 * ks + h), kf[ks], s);
+            dp = mma_rows<T>(L::row_frag(lg, 32 * t + (lane & 31), 2 * ks + h), vf[ks], dp);
+          }
+#pragma unroll
+          for (int g = 0; g < 4; g++) {
+            const f32x4 x = *(const f32x4*)(ll[buf] + 32 * t + 8 * g + 4 * h);
+            const f32x4 y = *(const f32x4*)(ld[buf] + 32 * t + 8 * g + 4 * h);
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+              weight<T, PLAIN>(a, s, dp, 4 * g + i, slope, cs, x[i], y[i],
+                               q0 + 32 * t + 4 * h + 8 * g + i - kj);
+          }
+          if (masked) {
+            const uint32_t see = visible<false>(band, lid + 32 * t, q0 + 32 * t, kj, kid, h);
+#pragma unroll
+            for (int r = 0; r < 16; r++) {
+              s[r] = (see >> r) & 1 ? s[r] : 0.0f;
+              dp[r] = (see >> r) & 1 ? dp[r] : 0.0f;
+            }
+          }
+          if (bad) {
+            cols_skipping<T, D>(dv, lg, 32 * t, s, lane);
+            cols_skipping<T, D>(dk, lq, 32 * t, dp, lane);
+          } else {
+            mma_cols<T, D>(dv, lg, 32 * t, s, lane);
+            mma_cols<T, D>(dk, lq, 32 * t, dp, lane);
+          }
+        }
+      };
+      while (qb >= 0) {
+        tile(lq0, lg0, 0, lq1, lg1);
+        if (qb < 0) break;
+        tile(lq1, lg1, 1, lq0, lg0);
+      }
+    }
+    if (kj < S) {
+      if constexpr (SPLIT) {
+        float* p = a.part + (((long)b * a.H + first) * S + kj) * D;
+        store_own<float, D>(p, dk, a.sigma, lane);
+        store_own<float, D>(p + (long)a.B * a.H * S * D, dv, 1.0f, lane);
+      } else {
+        store_own<T, D>((T*)a.dk + b * a.sdk[0] + hk * a.sdk[1] + kj * a.sdk[2], dk, a.sigma, lane);
+        store_own<T, D>((T*)a.dv + b * a.sdv[0] + hk * a.sdv[1] + kj * a.sdv[2], dv, 1.0f, lane);
+      }
+    }
+  }
+}
+
+// The sum of a group's partial dK and dV, heads ascending, four columns a thread.
+template <typename T, int D>
+__global__ void __launch_bounds__(256) mask_attn_join_kernel(const MaskAttnArgs a) {
+  const int group = a.H / a.Hkv;
+  const long n = (long)a.B * a.Hkv * a.S * (D / 4), half = (long)a.B * a.H * a.S * D;
+  for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < 2 * n; i += (long)gridDim.x * 256) {
+    const bool isv = i >= n;
+    long e = isv ? i - n : i;
+    const int d = (int)(e % (D / 4)) * 4;
+    e /= D / 4;
+    const int s = (int)(e % a.S);
+    e /= a.S;
+    const int hk = (int)(e % a.Hkv), b = (int)(e / a.Hkv);
+    const float* p = a.part + (isv ? half : 0) + (((long)b * a.H + hk * group) * a.S + s) * D + d;
+    float4 sum = *(const float4*)p;
+    for (int g = 1; g < group; g++) {
+      const float4 x = *(const float4*)(p + (long)g * a.S * D);
+      sum.x += x.x, sum.y += x.y, sum.z += x.z, sum.w += x.w;
+    }
+    T* o = isv ? (T*)a.dv + b * a.sdv[0] + hk * a.sdv[1] + s * a.sdv[2] + d
+               : (T*)a.dk + b * a.sdk[0] + hk * a.sdk[1] + s * a.sdk[2] + d;
+    o[0] = Elem<T>::put(sum.x), o[1] = Elem<T>::put(sum.y), o[2] = Elem<T>::put(sum.z), o[3] = Elem<T>::put(sum.w);
+  }
+}
+
+int grid_of(long work) { return (int)(work < (1 << 20) ? work : (1 << 20)); }
+
+}  // namespace
+
+// Whether dK/dV splits a group of query heads over workgroups.
+bool mask_attn_splits(int B, int H, int Hkv, int S) {
+  return H > Hkv && (long)B * Hkv * ((S + 127) / 128) < 2 * otx_cu_count();
+}
+
+hipError_t launch_mask_table(const int* doc, void* table, int B, int S, hipStream_t st) {
+  const int nb = (S + kTab - 1) / kTab;
+  mask_table_kernel<<<grid_of(((long)B * nb + 3) / 4), 256, 0, st>>>(doc, (i32x4*)table, B, S, nb);
+  return hipGetLastError();
+}
+
+template <typename T, int D, bool PLAIN>
+static hipError_t fwd_of(const MaskAttnArgs& a, hipStream_t st) {
+  mask_attn_fwd_kernel<T, D, PLAIN><<<grid_of((long)a.B * a.H * ((a.S + 127) / 128)), kThreads, 0, st>>>(a);
+  return hipGetLastError();
+}
+
+template <typename T, int D, bool PLAIN>
+static hipError_t bwd_of(const MaskAttnArgs& a, hipStream_t st) {
+  const long nt = (a.S + 127) / 128;
+  mask_attn_dq_kernel<T, D, PLAIN><<<grid_of((long)a.B * a.H * nt), kThreads, 0, st>>>(a);
+  if (a.part) {
+    mask_attn_dkdv_kernel<T, D, PLAIN, true><<<grid_of((long)a.B * a.H * nt), kThreads, 0, st>>>(a);
+    mask_attn_join_kernel<T, D><<<grid_of(((long)a.B * a.Hkv * a.S * (D / 2) + 255) / 256), 256, 0, st>>>(a);
+  } else {
+    mask_attn_dkdv_kernel<T, D, PLAIN, false><<<grid_of((long)a.B * a.Hkv * nt), kThreads, 0, st>>>(a);
+  }
+  return hipGetLastError();
+}
+
+hipError_t launch_mask_attn(int dtype, int D, bool backward, const MaskAttnArgs& a, hipStream_t st) {
+  const bool plain = !(a.cap > 0.0f) && !a.slopes;
+#define OTX_MA(T, DD) \
+  return backward ? (plain ? bwd_of<T, DD, true>(a, st) : bwd_of<T, DD, false>(a, st)) \
+                  : (plain ? fwd_of<T, DD, true>(a, st) : fwd_of<T, DD, false>(a, st));
+  if (dtype == 1) {
+    if (D == 64) OTX_MA(uint16_t, 64) else OTX_MA(uint16_t, 128)
+  }
+  if (D == 64) OTX_MA(float, 64) else OTX_MA(float, 128)
+#undef OTX_MA
+}
+
+}  // namespace otx

@@ -386,6 +386,203 @@ struct Attention : Function<Attention> {
   }
 };
 
+// Strides of b, h and s (or b, t and h) of a 4-D tensor as the C ABI takes them; those of
+// dimensions of one element say nothing and are left out.
+void put_strides(std::vector<long>& to, const Tensor& t, int d0 = 0, int d1 = 1, int d2 = 2) {
+  for (int d : {d0, d1, d2}) to.push_back(t.size(d) > 1 ? (long)t.stride(d) : 0);
+}
+
+// A tensor that kernels of 16-byte accesses can read through its strides, or a contiguous copy of it.
+Tensor rows16(const Tensor& t) {
+  const int64_t vec = 16 / t.element_size();
+  bool ok = (t.size(3) <= 1 || t.stride(3) == 1) && (uintptr_t)t.data_ptr() % 16 == 0;
+  for (int d = 0; d < 3; d++) ok = ok && (t.size(d) <= 1 || (t.stride(d) >= 0 && t.stride(d) % vec == 0));
+  ok = ok && (t.size(2) <= 1 || t.stride(2) < (1L << 22));
+  return ok ? t : t.clone(at::MemoryFormat::Contiguous);
+}
+
+// An empty tensor in t's order of dimensions, its rows contiguous.
+Tensor empty_rows(const Tensor& t) {
+  const Tensor r = at::empty_like(t);
+  return r.stride(3) == 1 ? r : at::empty(t.sizes(), t.options());
+}
+
+// q [B, H, S, D], k and v [B, Hkv, S, D], with any strides; slopes [H], doc_ids [B, S] and prefix [B]
+// contiguous, each or none.  Checked by nn/masked_attention.py.
+struct MaskedAttention : Function<MaskedAttention> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& q_, const Tensor& k_, const Tensor& v_,
+                        const std::optional<Tensor>& slopes, const std::optional<Tensor>& doc,
+                        const std::optional<Tensor>& prefix, int64_t window, double softcap) {
+    const Tensor q = rows16(q_), k = rows16(k_), v = rows16(v_);
+    const int B = (int)q.size(0), H = (int)q.size(1), Hkv = (int)k.size(1), S = (int)q.size(2), D = (int)q.size(3);
+    // in q's order of dimensions, so that the heads of a [B, S, H, D] projection merge without a copy
+    const Tensor o = empty_rows(q), lse = at::empty({B, H, S}, q.options().dtype(at::kFloat));
+    const Tensor table =
+        doc ? at::empty({(int64_t)otx_mask_attn_table_bytes(B, S) / 4}, q.options().dtype(at::kInt)) : Tensor();
+    std::vector<long> st;
+    for (const Tensor& t : {q, k, v, o}) put_strides(st, t);
+    {
+      Launch at(q);
+      check(otx_mask_attn_fwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), lse.data_ptr<float>(),
+                              slopes ? slopes->data_ptr<float>() : nullptr, doc ? doc->data_ptr<int>() : nullptr,
+                              prefix ? prefix->data_ptr<int>() : nullptr, doc ? table.data_ptr() : nullptr, st.data(),
+                              B, H, Hkv, S, D, (int)window, (float)softcap, dtype_code(q), at.stream),
+            "otx_mask_attn_fwd");
+    }
+    variable_list save = {q, k, v, o, lse};
+    if (slopes) save.push_back(*slopes);
+    if (prefix) save.push_back(*prefix);
+    if (doc) save.push_back(*doc), save.push_back(table);
+    ctx->save_for_backward(save);
+    ctx->saved_data["window"] = window;
+    ctx->saved_data["softcap"] = softcap;
+    ctx->saved_data["has"] = (int64_t)((slopes ? 1 : 0) | (prefix ? 2 : 0) | (doc ? 4 : 0));
+    return o;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    const Tensor dout = rows16(grads[0]);
+    const auto type = dout.scalar_type();
+    const int64_t B = dout.size(0), H = dout.size(1), S = dout.size(2), D = dout.size(3);
+    TORCH_CHECK_VALUE(saved[1].dim() == 4 && saved[1].size(1) > 0 && H % saved[1].size(1) == 0,
+                      "masked_attention: k came back from the saved tensors as ", saved[1].sizes());
+    const int64_t Hkv = saved[1].size(1), has = ctx->saved_data["has"].toInt();
+    // through their strides, which saved_as would lay out anew
+    auto strided = [&](const Tensor& t, at::IntArrayRef sizes, const char* what) {
+      TORCH_CHECK_VALUE(t.defined() && t.sizes() == sizes && t.scalar_type() == type && t.device() == dout.device(),
+                        "masked_attention: ", what, " came back from the saved tensors as ", t.toString(), t.sizes());
+      return rows16(t);
+    };
+    const Tensor q = strided(saved[0], {B, H, S, D}, "q"), k = strided(saved[1], {B, Hkv, S, D}, "k"),
+                 v = strided(saved[2], {B, Hkv, S, D}, "v"), o = strided(saved[3], {B, H, S, D}, "o");
+    const Tensor lse = saved_as(saved[4], {B, H, S}, at::kFloat, dout, "masked_attention: the logsumexp");
+    size_t at_ = 5;
+    Tensor slopes, prefix, doc, table;
+    if (has & 1) slopes = saved_as(saved[at_++], {H}, at::kFloat, dout, "masked_attention: slopes");
+    if (has & 2) prefix = saved_as(saved[at_++], {B}, at::kInt, dout, "masked_attention: prefix");
+    if (has & 4) {
+      doc = saved_as(saved[at_++], {B, S}, at::kInt, dout, "masked_attention: doc_ids");
+      table = saved_as(saved[at_++], {(int64_t)otx_mask_attn_table_bytes((int)B, (int)S) / 4}, at::kInt, dout,
+                       "masked_attention: the block table");
+    }
+    const Tensor dq = empty_rows(q), dk = empty_rows(k), dv = empty_rows(v);
+    std::vector<long> st;
+    for (const Tensor& t : {q, k, v, o, dout, dq, dk, dv}) put_strides(st, t);
+    Launch at(q);
+    const size_t nbytes = otx_mask_attn_bwd_workspace_bytes((int)B, (int)H, (int)Hkv, (int)S, (int)D);
+    const Workspace ws(q, nbytes);
+    check(otx_mask_attn_bwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), lse.data_ptr<float>(),
+                            dout.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
+                            has & 1 ? slopes.data_ptr<float>() : nullptr, has & 4 ? doc.data_ptr<int>() : nullptr,
+                            has & 2 ? prefix.data_ptr<int>() : nullptr, has & 4 ? table.data_ptr() : nullptr, st.data(),
+                            (int)B, (int)H, (int)Hkv, (int)S, (int)D, (int)ctx->saved_data["window"].toInt(),
+                            (float)ctx->saved_data["softcap"].toDouble(), dtype_code(q), ws.ptr, nbytes, at.stream),
+          "otx_mask_attn_bwd");
+    return {dq, dk, dv, Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
+  }
+};
+
+// x [B, T, H, D] (strides as they are, the last 1) -> [B, H, T, D], and back with the transposed turn.
+Tensor rotate(const Tensor& x, const Tensor& cos, const Tensor& sin, const std::optional<Tensor>& positions,
+              int64_t layout, bool backward) {
+  const int64_t B = x.size(0), D = x.size(3), T = x.size(backward ? 2 : 1), H = x.size(backward ? 1 : 2);
+  const Tensor xc = D == 1 || x.stride(3) == 1 ? x : x.contiguous();
+  const Tensor y = backward ? at::empty({B, T, H, D}, x.options()) : at::empty({B, H, T, D}, x.options());
+  std::vector<long> st;
+  if (backward)
+    put_strides(st, xc, 0, 2, 1), put_strides(st, y);
+  else
+    put_strides(st, xc), put_strides(st, y, 0, 2, 1);
+  Launch at(x);
+  check(otx_rotary(xc.data_ptr(), cos.data_ptr<float>(), sin.data_ptr<float>(),
+                   positions ? positions->data_ptr<int>() : nullptr, y.data_ptr(), st.data(), (int)B, (int)T, (int)H,
+                   (int)D, (int)cos.size(1) * 2, (int)cos.size(0), (int)layout, backward ? 1 : 0, dtype_code(x),
+                   at.stream),
+        "otx_rotary");
+  return y;
+}
+
+struct RotaryHeads : Function<RotaryHeads> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& cos, const Tensor& sin,
+                        const std::optional<Tensor>& positions, int64_t layout) {
+    const Tensor y = rotate(x, cos, sin, positions, layout, false);
+    variable_list save = {cos, sin};
+    if (positions) save.push_back(*positions);
+    ctx->save_for_backward(save);
+    ctx->saved_data["layout"] = layout;
+    ctx->saved_data["P"] = cos.size(0);
+    ctx->saved_data["half"] = cos.size(1);
+    return y;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    const Tensor dy = grads[0];
+    const int64_t P = ctx->saved_data["P"].toInt(), n = ctx->saved_data["half"].toInt();
+    const Tensor cos = saved_as(saved[0], {P, n}, at::kFloat, dy, "rotary_heads: cos");
+    const Tensor sin = saved_as(saved[1], {P, n}, at::kFloat, dy, "rotary_heads: sin");
+    std::optional<Tensor> positions;
+    if (saved.size() > 2)
+      positions = saved_as(saved[2], {dy.size(0), dy.size(2)}, at::kInt, dy, "rotary_heads: positions");
+    return {rotate(dy, cos, sin, positions, ctx->saved_data["layout"].toInt(), true), Tensor(), Tensor(), Tensor(),
+            Tensor()};
+  }
+};
+
+struct LayerNorm : Function<LayerNorm> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& w, const std::optional<Tensor>& b,
+                        double eps) {
+    const int64_t D = x.size(-1);
+    check_device(w, x, "layer_norm: the weight");
+    TORCH_CHECK_VALUE(D > 0 && D <= INT_MAX, "layer_norm: last dimension of ", D);
+    TORCH_CHECK_VALUE(w.numel() == D, "layer_norm: weight ", w.sizes(), " for an input of width ", D);
+    if (b) {
+      check_device(*b, x, "layer_norm: the bias");
+      TORCH_CHECK_VALUE(b->numel() == D, "layer_norm: bias ", b->sizes(), " for an input of width ", D);
+      TORCH_CHECK_VALUE(b->scalar_type() == w.scalar_type(), "layer_norm: a ", b->scalar_type(), " bias beside a ",
+                        w.scalar_type(), " weight");
+    }
+    dtype_code(w);
+    const Tensor xc = x.contiguous(), wc = w.to(x.scalar_type()).contiguous();
+    const Tensor bc = b ? b->to(x.scalar_type()).contiguous() : Tensor();
+    const int64_t rows = xc.numel() / D;
+    const Tensor y = at::empty_like(xc), stats = at::empty({2, rows}, x.options().dtype(at::kFloat));
+    {
+      Launch at(x);
+      float* mean = stats.data_ptr<float>();
+      check(otx_layer_norm_fwd(xc.data_ptr(), wc.data_ptr(), b ? bc.data_ptr() : nullptr, y.data_ptr(), mean,
+                               mean + rows, rows, (int)D, (float)eps, dtype_code(x), at.stream),
+            "otx_layer_norm_fwd");
+    }
+    ctx->save_for_backward({xc, wc, stats});
+    ctx->saved_data["wdtype"] = (int64_t)w.scalar_type();
+    ctx->saved_data["wshape"] = w.sizes().vec();
+    if (b) ctx->saved_data["bshape"] = b->sizes().vec();
+    return y;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    const Tensor dy = grads[0].contiguous();
+    const int64_t D = dy.size(-1), rows = dy.numel() / D;
+    const Tensor x = saved_as(saved[0], dy.sizes(), dy.scalar_type(), dy, "layer_norm: the input");
+    TORCH_CHECK_VALUE(saved[1].numel() == D, "layer_norm: the weight came back as ", saved[1].sizes());
+    const Tensor w = saved_as(saved[1], saved[1].sizes(), dy.scalar_type(), dy, "layer_norm: the weight");
+    const Tensor stats = saved_as(saved[2], {2, rows}, at::kFloat, dy, "layer_norm: the row statistics");
+    const auto wtype = (at::ScalarType)ctx->saved_data["wdtype"].toInt();
+    const bool bias = ctx->saved_data.count("bshape") != 0;
+    const Tensor dx = at::empty_like(x), dw = at::empty(ctx->saved_data["wshape"].toIntVector(), x.options().dtype(wtype));
+    const Tensor db = bias ? at::empty(ctx->saved_data["bshape"].toIntVector(), x.options().dtype(wtype)) : Tensor();
+    Launch at(x);
+    const size_t nbytes = otx_layer_norm_bwd_workspace_bytes(rows, (int)D);
+    const Workspace ws(x, nbytes);
+    const float* mean = stats.data_ptr<float>();
+    check(otx_layer_norm_bwd(x.data_ptr(), w.data_ptr(), mean, mean + rows, dy.data_ptr(), dx.data_ptr(),
+                             dw.data_ptr(), bias ? db.data_ptr() : nullptr, rows, (int)D, dtype_code(x),
+                             dtype_code(dw), ws.ptr, nbytes, at.stream),
+          "otx_layer_norm_bwd");
+    return {dx, dw, db, Tensor()};
+  }
+};
+
 Tensor linear(const Tensor& x, const Tensor& w) { return Linear::apply(x, w); }
 Tensor rms_norm(const Tensor& x, const Tensor& w, double eps) { return RMSNorm::apply(x, w, eps); }
 Tensor silu(const Tensor& x) { return SiLU::apply(x); }
@@ -400,6 +597,18 @@ std::tuple<Tensor, Tensor> loss(const Tensor& logits, const Tensor& labels, doub
 Tensor attention(const Tensor& q, const Tensor& k, const Tensor& v, const std::optional<Tensor>& sc, int64_t window,
                  bool int8pv) {
   return Attention::apply(q, k, v, sc, window, int8pv);
+}
+Tensor masked_attention(const Tensor& q, const Tensor& k, const Tensor& v, const std::optional<Tensor>& slopes,
+                        const std::optional<Tensor>& doc, const std::optional<Tensor>& prefix, int64_t window,
+                        double softcap) {
+  return MaskedAttention::apply(q, k, v, slopes, doc, prefix, window, softcap);
+}
+Tensor rotary_heads(const Tensor& x, const Tensor& cos, const Tensor& sin, const std::optional<Tensor>& positions,
+                    int64_t layout) {
+  return RotaryHeads::apply(x, cos, sin, positions, layout);
+}
+Tensor layer_norm(const Tensor& x, const Tensor& w, const std::optional<Tensor>& b, double eps) {
+  return LayerNorm::apply(x, w, b, eps);
 }
 
 }  // namespace
@@ -416,4 +625,7 @@ PYBIND11_MODULE(_otx_autograd, m) {
   m.def("embedding", torch::wrap_pybind_function(embedding));
   m.def("loss", torch::wrap_pybind_function(loss));
   m.def("attention", torch::wrap_pybind_function(attention));
+  m.def("masked_attention", torch::wrap_pybind_function(masked_attention));
+  m.def("rotary_heads", torch::wrap_pybind_function(rotary_heads));
+  m.def("layer_norm", torch::wrap_pybind_function(layer_norm));
 }

@@ -9,6 +9,7 @@
 #include <cstdarg>
 #include <cstring>
 #include <mutex>
+#include "otx_args.h"
 #include "otx_common.h"
 #include "../../include/otx_attn.h"
 
@@ -46,6 +47,16 @@ hipError_t launch_swiglu(int dtype, int backward, const void* gu, const void* dh
 hipError_t launch_rope_heads(int dtype, int backward, const void* in, const float* cosv, const float* sinv, void* out,
                              int B, int Tn, int H, int D, hipStream_t st);
 hipError_t launch_swap_heads(int dtype, const void* in, void* out, int B, int X, int Y, int D, hipStream_t st);
+bool mask_attn_splits(int B, int H, int Hkv, int S);
+hipError_t launch_mask_table(const int* doc, void* table, int B, int S, hipStream_t st);
+hipError_t launch_mask_attn(int dtype, int D, bool backward, const MaskAttnArgs& a, hipStream_t st);
+hipError_t launch_rotary(int dtype, const RotaryArgs& a, bool half, bool wide, hipStream_t st);
+int layer_norm_parts(long rows, int D);
+hipError_t launch_layer_norm_fwd(int dtype, bool wide, const void* x, const void* w, const void* b, void* y,
+                                 float* mean, float* rstd, long rows, int D, float eps, hipStream_t st);
+hipError_t launch_layer_norm_bwd(int dtype, bool wide, const void* x, const void* w, const float* mean,
+                                 const float* rstd, const void* dy, void* dx, void* dw, void* db, int wdtype,
+                                 float* part, long rows, int D, hipStream_t st);
 }  // namespace otx
 
 static thread_local char g_err[512];
@@ -774,6 +785,174 @@ int otx_embedding_bwd(const int64_t* ids, const void* grad_out, void* grad_weigh
                                      workspace_bytes - emb_arrays_bytes(npos), (hipStream_t)stream);
   if (e != hipSuccess) return fail(OTX_EHIP, "embedding backward launch failed: %s", hipGetErrorString(e));
   return OTX_OK;
+}
+
+}  // extern "C"
+
+// ---- masked attention ----
+
+static int check_mask_shape(int B, int H, int Hkv, int S, int D) {
+  if (B <= 0 || H <= 0 || Hkv <= 0 || S <= 0) return fail(OTX_EINVAL, "B, H, Hkv and S must be positive");
+  if (H % Hkv != 0) return fail(OTX_EINVAL, "H (%d) must be a multiple of Hkv (%d)", H, Hkv);
+  if (D != 64 && D != 128) return fail(OTX_EINVAL, "head_dim %d not supported (64 or 128)", D);
+  if (S > (1 << 24)) return fail(OTX_EINVAL, "sequence length %d exceeds 2^24", S);
+  if ((long long)B * H > 0x7fffffffLL || (long long)B * H * S * D >= (1LL << 40))
+    return fail(OTX_EINVAL, "tensor too large");
+  return OTX_OK;
+}
+
+// Strides of b, h and s of one tensor; rows have to start at 16-byte boundaries.
+static int mask_strides(const char* name, const void* p, const long* in, int dtype, long* out) {
+  const long vec = dtype == OTX_DTYPE_BF16 ? 8 : 4;
+  if (!p) return fail(OTX_EINVAL, "null pointer argument: %s", name);
+  if (!aligned16(p)) return fail(OTX_EINVAL, "%s must be 16-byte aligned", name);
+  for (int i = 0; i < 3; i++) {
+    if (in[i] < 0 || in[i] % vec)
+      return fail(OTX_EINVAL, "%s: stride %ld is not a non-negative multiple of %ld elements", name, in[i], vec);
+    out[i] = in[i];
+  }
+  if (in[2] >= (1L << 22)) return fail(OTX_EINVAL, "%s: row stride %ld too large", name, in[2]);
+  return OTX_OK;
+}
+
+static int mask_args(otx::MaskAttnArgs* a, const float* slopes, const int32_t* doc_ids, const int32_t* prefix,
+                     void* table, int B, int H, int Hkv, int S, int D, int window, float softcap, int dtype) {
+  int rc = check_mask_shape(B, H, Hkv, S, D);
+  if (rc) return rc;
+  if (dtype != OTX_DTYPE_F32 && dtype != OTX_DTYPE_BF16) return fail(OTX_EINVAL, "dtype code %d not supported", dtype);
+  if (window < 0) return fail(OTX_EINVAL, "window %d must not be negative", window);
+  if (!(softcap >= 0.0f && softcap <= 3e38f)) return fail(OTX_EINVAL, "softcap %g must be 0 or positive", (double)softcap);
+  if (doc_ids && (!table || !aligned16(table))) return fail(OTX_EINVAL, "doc_ids need a 16-byte aligned block table");
+  a->slopes = slopes, a->doc = doc_ids, a->prefix = prefix, a->table = table;
+  a->B = B, a->H = H, a->Hkv = Hkv, a->S = S;
+  a->window = window >= S ? 0 : window;
+  a->sigma = otx_softmax_scale(D), a->cap = softcap;
+  return OTX_OK;
+}
+
+extern "C" {
+
+size_t otx_mask_attn_table_bytes(int B, int S) {
+  if (B <= 0 || S <= 0) return 0;
+  return (size_t)B * (((size_t)S + 63) / 64) * 16;
+}
+
+static size_t mask_dsum_bytes(int B, int H, int S) { return ((size_t)B * H * S * 4 + 255) / 256 * 256; }
+
+size_t otx_mask_attn_bwd_workspace_bytes(int B, int H, int Hkv, int S, int D) {
+  if (check_mask_shape(B, H, Hkv, S, D) != OTX_OK) return 0;
+  return mask_dsum_bytes(B, H, S) + (otx::mask_attn_splits(B, H, Hkv, S) ? (size_t)B * H * S * D * 8 : 0);
+}
+
+int otx_mask_attn_fwd(const void* q, const void* k, const void* v, void* o, float* lse, const float* slopes,
+                      const int32_t* doc_ids, const int32_t* prefix, void* table, const long* strides, int B, int H,
+                      int Hkv, int S, int D, int window, float softcap, int dtype, void* stream) {
+  otx::MaskAttnArgs a = {};
+  int rc = mask_args(&a, slopes, doc_ids, prefix, table, B, H, Hkv, S, D, window, softcap, dtype);
+  if (rc) return rc;
+  if (!strides || !lse) return fail(OTX_EINVAL, "null pointer argument");
+  if ((rc = mask_strides("q", q, strides, dtype, a.sq)) || (rc = mask_strides("k", k, strides + 3, dtype, a.sk)) ||
+      (rc = mask_strides("v", v, strides + 6, dtype, a.sv)) || (rc = mask_strides("o", o, strides + 9, dtype, a.so)))
+    return rc;
+  a.q = q, a.k = k, a.v = v, a.out = o, a.lse = lse;
+  hipError_t e = doc_ids ? otx::launch_mask_table(doc_ids, table, B, S, (hipStream_t)stream) : hipSuccess;
+  if (e == hipSuccess) e = otx::launch_mask_attn(dtype, D, false, a, (hipStream_t)stream);
+  return e == hipSuccess ? OTX_OK : fail(OTX_EHIP, "masked attention launch failed: %s", hipGetErrorString(e));
+}
+
+int otx_mask_attn_bwd(const void* q, const void* k, const void* v, const void* o, const float* lse, const void* dout,
+                      void* dq, void* dk, void* dv, const float* slopes, const int32_t* doc_ids, const int32_t* prefix,
+                      const void* table, const long* strides, int B, int H, int Hkv, int S, int D, int window,
+                      float softcap, int dtype, void* workspace, size_t workspace_bytes, void* stream) {
+  otx::MaskAttnArgs a = {};
+  int rc = mask_args(&a, slopes, doc_ids, prefix, (void*)table, B, H, Hkv, S, D, window, softcap, dtype);
+  if (rc) return rc;
+  if (!strides || !lse || !workspace) return fail(OTX_EINVAL, "null pointer argument");
+  if ((rc = mask_strides("q", q, strides, dtype, a.sq)) || (rc = mask_strides("k", k, strides + 3, dtype, a.sk)) ||
+      (rc = mask_strides("v", v, strides + 6, dtype, a.sv)) || (rc = mask_strides("o", o, strides + 9, dtype, a.so)) ||
+      (rc = mask_strides("dout", dout, strides + 12, dtype, a.sdo)) ||
+      (rc = mask_strides("dq", dq, strides + 15, dtype, a.sdq)) ||
+      (rc = mask_strides("dk", dk, strides + 18, dtype, a.sdk)) ||
+      (rc = mask_strides("dv", dv, strides + 21, dtype, a.sdv)))
+    return rc;
+  if ((uintptr_t)workspace & 255u) return fail(OTX_EINVAL, "the workspace must be 256-byte aligned");
+  const size_t need = otx_mask_attn_bwd_workspace_bytes(B, H, Hkv, S, D);
+  if (workspace_bytes < need)
+    return fail(OTX_EINVAL, "workspace too small: %zu bytes given, %zu needed", workspace_bytes, need);
+  a.q = q, a.k = k, a.v = v, a.o = o, a.lse = (float*)lse, a.dout = dout, a.dq = dq, a.dk = dk, a.dv = dv;
+  a.dsum = (float*)workspace;
+  if (otx::mask_attn_splits(B, H, Hkv, S)) a.part = (float*)((char*)workspace + mask_dsum_bytes(B, H, S));
+  hipError_t e = otx::launch_mask_attn(dtype, D, true, a, (hipStream_t)stream);
+  return e == hipSuccess ? OTX_OK : fail(OTX_EHIP, "masked attention backward launch failed: %s", hipGetErrorString(e));
+}
+
+// ---- rotary positions ----
+
+int otx_rotary(const void* x, const float* cosv, const float* sinv, const int32_t* positions, void* y,
+               const long* strides, int B, int T, int H, int D, int R, int P, int layout, int backward, int dtype,
+               void* stream) {
+  if (B <= 0 || T <= 0 || H <= 0 || D <= 0) return fail(OTX_EINVAL, "rotary: B, T, H and D must be positive");
+  if (R < 2 || R % 2 || R > D) return fail(OTX_EINVAL, "rotary: %d rotated columns of %d (an even number, at least 2)", R, D);
+  if (P <= 0 || (!positions && T > P)) return fail(OTX_EINVAL, "rotary: tables of %d positions for %d rows", P, T);
+  if (layout != 0 && layout != 1) return fail(OTX_EINVAL, "rotary: layout %d (0 interleaved, 1 half)", layout);
+  if (dtype != OTX_DTYPE_F32 && dtype != OTX_DTYPE_BF16) return fail(OTX_EINVAL, "dtype code %d not supported", dtype);
+  if (!x || !cosv || !sinv || !y || !strides) return fail(OTX_EINVAL, "null pointer argument");
+  if (x == y) return fail(OTX_EINVAL, "rotary: the output must not alias the input");
+  if (D > (1 << 20) || H > 65535 || (long long)B * T * (D / 2 + 1) >= 0x80000000LL)
+    return fail(OTX_EINVAL, "rotary: tensor too large");
+  const int vec = dtype == OTX_DTYPE_BF16 ? 8 : 4;
+  otx::RotaryArgs a = {};
+  bool wide = D % vec == 0 && R % (2 * vec) == 0 && aligned16(x) && aligned16(y) && aligned16(cosv) && aligned16(sinv);
+  for (int i = 0; i < 3; i++) {
+    a.sx[i] = strides[i], a.sy[i] = strides[3 + i];
+    if (a.sx[i] < 0 || a.sy[i] < 0) return fail(OTX_EINVAL, "rotary: negative stride");
+    wide = wide && a.sx[i] % vec == 0 && a.sy[i] % vec == 0;
+  }
+  a.x = x, a.y = y, a.cosv = cosv, a.sinv = sinv, a.positions = positions;
+  a.B = B, a.T = T, a.H = H, a.D = D, a.R = R, a.P = P, a.sign = backward ? -1.0f : 1.0f;
+  hipError_t e = otx::launch_rotary(dtype, a, layout == 1, wide, (hipStream_t)stream);
+  return e == hipSuccess ? OTX_OK : fail(OTX_EHIP, "rotary launch failed: %s", hipGetErrorString(e));
+}
+
+// ---- layer norm ----
+
+static int check_layer_norm(long rows, int D, int dtype) {
+  if (rows <= 0 || D <= 0) return fail(OTX_EINVAL, "layer norm: rows and width must be positive");
+  if (D > (1 << 24) || rows > 0x7fffffffL) return fail(OTX_EINVAL, "layer norm: %ld rows of %d columns too large", rows, D);
+  if (dtype != OTX_DTYPE_F32 && dtype != OTX_DTYPE_BF16) return fail(OTX_EINVAL, "dtype code %d not supported", dtype);
+  return OTX_OK;
+}
+
+int otx_layer_norm_fwd(const void* x, const void* w, const void* b, void* y, float* mean, float* rstd, long rows, int D,
+                       float eps, int dtype, void* stream) {
+  int rc = check_layer_norm(rows, D, dtype);
+  if (rc) return rc;
+  if (!x || !w || !y || !mean || !rstd) return fail(OTX_EINVAL, "null pointer argument");
+  const bool wide = D % (dtype == OTX_DTYPE_BF16 ? 8 : 4) == 0 && aligned16(x) && aligned16(w) && aligned16(b) && aligned16(y);
+  hipError_t e = otx::launch_layer_norm_fwd(dtype, wide, x, w, b, y, mean, rstd, rows, D, eps, (hipStream_t)stream);
+  return e == hipSuccess ? OTX_OK : fail(OTX_EHIP, "layer norm launch failed: %s", hipGetErrorString(e));
+}
+
+size_t otx_layer_norm_bwd_workspace_bytes(long rows, int D) {
+  if (check_layer_norm(rows, D, OTX_DTYPE_F32) != OTX_OK) return 0;
+  return (size_t)otx::layer_norm_parts(rows, D) * D * 2 * sizeof(float);
+}
+
+int otx_layer_norm_bwd(const void* x, const void* w, const float* mean, const float* rstd, const void* dy, void* dx,
+                       void* dw, void* db, long rows, int D, int dtype, int wdtype, void* workspace,
+                       size_t workspace_bytes, void* stream) {
+  int rc = check_layer_norm(rows, D, dtype);
+  if (rc) return rc;
+  if (wdtype != OTX_DTYPE_F32 && wdtype != OTX_DTYPE_BF16) return fail(OTX_EINVAL, "dtype code %d not supported", wdtype);
+  if (!x || !w || !mean || !rstd || !dy || !dx || !dw || !workspace) return fail(OTX_EINVAL, "null pointer argument");
+  if (!aligned16(workspace)) return fail(OTX_EINVAL, "the workspace must be 16-byte aligned");
+  const size_t need = otx_layer_norm_bwd_workspace_bytes(rows, D);
+  if (workspace_bytes < need)
+    return fail(OTX_EINVAL, "workspace too small: %zu bytes given, %zu needed", workspace_bytes, need);
+  const bool wide = D % (dtype == OTX_DTYPE_BF16 ? 8 : 4) == 0 && aligned16(x) && aligned16(w) && aligned16(dy) && aligned16(dx);
+  hipError_t e = otx::launch_layer_norm_bwd(dtype, wide, x, w, mean, rstd, dy, dx, dw, db, wdtype, (float*)workspace,
+                                            rows, D, (hipStream_t)stream);
+  return e == hipSuccess ? OTX_OK : fail(OTX_EHIP, "layer norm backward launch failed: %s", hipGetErrorString(e));
 }
 
 }  // extern "C"

@@ -10,6 +10,9 @@ and the torch compositions around them, each fused into one pass:
                         (rope.py:103-125, attention_repop.py:143-149)
   heads(x)              x.transpose(1, 2).contiguous() (attention_repop.py:150)
   merge_heads(o)        o.transpose(1, 2).contiguous().view(B, T, H * D) (attention_repop.py:155)
+and two operators without a repop counterpart, in binary32 with one rounding per result:
+  layer_norm(x, w, b)   LayerNorm over the last dimension
+  rotary_heads(x, c, s) rope_heads for either pair layout, part of the head and gathered positions
 Each is an autograd node of csrc/otx_autograd.cpp over the C ABI of libotx_attn.so: bf16 in,
 binary32 arithmetic in a fixed order, bf16 out, and for the compositions the
 bytes torch's own forward and autograd backward give; weight gradients come
@@ -23,7 +26,8 @@ import torch
 from .. import _lib
 from . import _nodes
 
-__all__ = ["linear", "rms_norm", "silu", "swiglu", "rope_heads", "heads", "merge_heads"]
+__all__ = ["linear", "rms_norm", "silu", "swiglu", "rope_heads", "heads", "merge_heads", "layer_norm",
+           "rotary_heads"]
 
 _DT = {torch.bfloat16: _lib.DTYPE_BF16, torch.float32: _lib.DTYPE_F32}
 
@@ -119,3 +123,53 @@ def merge_heads(o: torch.Tensor) -> torch.Tensor:
                          f"{o.dtype} {tuple(o.shape)}")
     B, H, T, D = o.shape
     return _nodes.call("swap_heads", o).view(B, T, H * D)
+
+
+def layer_norm(x: torch.Tensor, w: torch.Tensor, b: torch.Tensor | None = None, eps: float = 1e-5) -> torch.Tensor:
+    """Layer norm over the last dimension, of any width: (x - mean) / sqrt(var + eps) * w + b, in x's dtype.
+    The gradients of w and b come back in their dtype."""
+    _need_gpu(x, w, *(() if b is None else (b,)))
+    if x.dtype not in _DT:
+        raise ValueError(f"dtype {x.dtype} not supported")
+    if x.dim() == 0 or x.numel() == 0:
+        raise ValueError(f"layer_norm: empty input {tuple(x.shape)}")
+    return _nodes.call("layer_norm", x, w, b, float(eps))
+
+
+_PAIRS = {"interleaved": 0, "half": 1}
+
+
+def rotary_heads(x: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, positions: torch.Tensor | None = None,
+                 layout: str = "half") -> torch.Tensor:
+    """Rotary positions of x [B, T, H, D] into the attention layout [B, H, T, D].
+
+    cos and sin are binary32 [P, R / 2] (rope.rope_tables, rope.scaled_rope_tables), R <= D: columns 0 .. R - 1 are
+    turned in pairs (i, i + R / 2) (``layout`` "half") or (2 i, 2 i + 1) ("interleaved"), the others are copied.
+    Row t takes position positions[b, t] (int32 [B, T]), or t without them; a position outside 0 .. P - 1 makes
+    its row's turned columns NaN.  x may be a view with a contiguous last dimension.  Binary32 arithmetic, one rounding."""
+    _need_gpu(x, cos, sin, *(() if positions is None else (positions,)))
+    if x.dtype not in _DT:
+        raise ValueError(f"dtype {x.dtype} not supported")
+    if x.dim() != 4 or x.numel() == 0:
+        raise ValueError(f"rotary_heads takes x [B, T, H, D], got {tuple(x.shape)}")
+    if layout not in _PAIRS:
+        raise ValueError(f"layout {layout!r} is not one of {sorted(_PAIRS)}")
+    B, T, _, D = x.shape
+    for name, t in (("cos", cos), ("sin", sin)):
+        if t.dtype != torch.float32 or t.dim() != 2 or t.shape != cos.shape:
+            raise ValueError(f"rotary_heads: {name} must be binary32 [P, R / 2] as cos is, got {t.dtype} {tuple(t.shape)}")
+        if t.requires_grad:
+            raise ValueError(f"rotary_heads: {name} is a constant of this operator and gets no gradient: detach it")
+    P, half = cos.shape
+    if not 1 <= half <= D // 2:
+        raise ValueError(f"rotary_heads: tables of {half} pairs for heads of {D} columns")
+    if positions is None:
+        if T > P:
+            raise ValueError(f"rotary_heads: {T} rows, tables of {P} positions")
+    elif positions.dtype != torch.int32 or tuple(positions.shape) != (B, T):
+        raise ValueError(f"rotary_heads: positions must be int32 [{B}, {T}], got {positions.dtype} {tuple(positions.shape)}")
+    for name, t in (("cos", cos), ("sin", sin), ("positions", positions)):
+        if t is not None and t.device != x.device:
+            raise RuntimeError(f"rotary_heads: {name} is on {t.device}, x on {x.device}")
+    return _nodes.call("rotary_heads", x, cos.contiguous(), sin.contiguous(),
+                       None if positions is None else positions.contiguous(), _PAIRS[layout])

@@ -114,3 +114,43 @@ def _tables(seq_len: int, head_dim: int, theta: float) -> tuple[np.ndarray, np.n
 def rope_tables(seq_len: int, head_dim: int, theta: float) -> tuple[np.ndarray, np.ndarray]:
     """cos, sin tables [seq_len, head_dim/2] (binary32, read-only arrays)."""
     return _tables(int(seq_len), int(head_dim), float(theta))
+
+
+def scaled_rope_tables(seq_len: int, rotary_dim: int, theta: float, factor: float = 1.0, method: str = "linear",
+                       original_len: int | None = None, beta_fast: float = 32.0, beta_slow: float = 1.0,
+                       attention_factor: float | None = None) -> tuple[np.ndarray, np.ndarray]:
+    """cos, sin tables [seq_len, rotary_dim / 2] (binary32) for a context stretched by ``factor``.
+
+    ``linear``: positions divided by factor (position interpolation).  ``yarn``: frequencies that turn more than
+    beta_fast times over original_len are kept, those that turn less than beta_slow times are divided by factor, in
+    between the two are blended linearly over the index of the frequency; both tables are multiplied by
+    attention_factor, by default 0.1 ln(factor) + 1 (Peng et al., "YaRN: Efficient Context Window Extension of Large
+    Language Models", 2023).  Angles are formed in binary64, so that far positions keep their phase, and each entry
+    is rounded to binary32 once.
+    """
+    if seq_len < 1 or rotary_dim < 2 or rotary_dim % 2:
+        raise ValueError(f"tables of {seq_len} positions and {rotary_dim} rotated columns")
+    if not factor >= 1.0 or not np.isfinite(factor):
+        raise ValueError(f"factor {factor} must be at least 1")
+    freq = theta ** (-np.arange(0, rotary_dim, 2, dtype=np.float64) / rotary_dim)
+    scale = 1.0
+    if method == "linear":
+        freq = freq / factor
+        scale = 1.0 if attention_factor is None else attention_factor
+    elif method == "yarn":
+        if not original_len or original_len < 1:
+            raise ValueError("yarn needs original_len, the context that the model was trained on")
+        if not beta_fast > beta_slow > 0:
+            raise ValueError(f"beta_fast {beta_fast} must exceed beta_slow {beta_slow}, which must be positive")
+
+        def index(turns: float) -> float:  # of the frequency that turns so often over original_len
+            return rotary_dim * np.log(original_len / (turns * 2 * np.pi)) / (2 * np.log(theta))
+
+        low, high = max(np.floor(index(beta_fast)), 0.0), min(np.ceil(index(beta_slow)), rotary_dim - 1.0)
+        stretched = np.clip((np.arange(rotary_dim // 2) - low) / max(high - low, 1e-3), 0.0, 1.0)
+        freq = freq * (1 - stretched) + freq / factor * stretched
+        scale = 0.1 * np.log(factor) + 1.0 if attention_factor is None else attention_factor
+    else:
+        raise ValueError(f"method {method!r} is not 'linear' or 'yarn'")
+    angle = np.arange(seq_len, dtype=np.float64)[:, None] * freq[None, :]
+    return (scale * np.cos(angle)).astype(_F32), (scale * np.sin(angle)).astype(_F32)

@@ -1,0 +1,273 @@
+"""rotary_heads and layer_norm on the GPU against binary64, with bounds counted in half steps of the types."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from open_transformers_amd import rope
+from open_transformers_amd.nn import functional as F
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+BF, F32 = torch.bfloat16, torch.float32
+U = 2.0**-24
+
+
+def within(name, got, value, bound):
+    got = got.detach().double().cpu()
+    assert got.shape == value.shape, (got.shape, value.shape)
+    assert torch.isfinite(got).all(), name
+    off = (got - value).abs() / (bound + 1e-30)
+    assert off.max() <= 1, f"{name}: {float(off.max()):.3g} times the bound, at {torch.nonzero(off > 1)[:4].tolist()}"
+
+
+# ---- rotary -------------------------------------------------------------------------------------------------------
+
+def turned(x, cos, sin, at, layout, back=False):
+    """x [B, H, T, D] in binary64, and the sum of the magnitudes that make up each result."""
+    R = 2 * cos.shape[1]
+    c, s = cos.double()[at][:, None], sin.double()[at][:, None] * (-1 if back else 1)
+    a, b = (slice(0, R // 2), slice(R // 2, R)) if layout == "half" else (slice(0, R, 2), slice(1, R, 2))
+    y, size = x.clone(), x.abs()
+    y[..., a], y[..., b] = x[..., a] * c - x[..., b] * s, x[..., a] * s + x[..., b] * c
+    size[..., a] = (x[..., a] * c).abs() + (x[..., b] * s).abs()
+    size[..., b] = (x[..., a] * s).abs() + (x[..., b] * c).abs()
+    return y, size
+
+
+ROTARY = [
+    # dtype, B, T, H, D, R, positions
+    (BF, 1, 1, 1, 64, 64, True), (F32, 2, 3, 2, 2, 2, True), (BF, 2, 61, 16, 128, 128, True),
+    (BF, 1, 130, 3, 128, 32, False), (F32, 2, 77, 5, 96, 24, True), (F32, 1, 33, 4, 80, 80, False),
+    (BF, 1, 20, 3, 37, 10, True), (F32, 1, 9, 2, 130, 64, True), (BF, 3, 50, 1, 256, 128, True),
+    (BF, 1, 700, 9, 72, 48, False), (BF, 2, 19, 3, 80, 16, False),
+]
+
+
+@pytest.mark.parametrize("layout", ["half", "interleaved"])
+@pytest.mark.parametrize("dtype,B,T,H,D,R,gather", ROTARY)
+def test_rotary(dtype, B, T, H, D, R, gather, layout):
+    gen = torch.Generator().manual_seed(T + D)
+    P = T + 11
+    cos, sin = (torch.from_numpy(t) for t in rope.scaled_rope_tables(P, R, 1e4, 4.0, "yarn", original_len=16))
+    x = torch.randn(B, T, H, D, generator=gen).to(dtype)
+    dy = torch.randn(B, H, T, D, generator=gen).to(dtype)
+    at = torch.randint(0, P, (B, T), generator=gen) if gather else torch.arange(T).expand(B, T)
+    half = torch.finfo(dtype).eps / 2
+    for view in (False, True):
+        leaf = x.to(DEV).requires_grad_()
+        given = torch.cat([torch.zeros_like(leaf), leaf], 2)[:, :, H:] if view else leaf
+        y = F.rotary_heads(given, cos.to(DEV), sin.to(DEV), positions=at.int().to(DEV) if gather else None, layout=layout)
+        assert y.is_contiguous()
+        (dx,) = torch.autograd.grad(y, leaf, dy.to(DEV))
+        value, size = turned(x.double().transpose(1, 2), cos, sin, at, layout)
+        within("y", y, value, half * value.abs() + 3 * U * size)
+        value, size = turned(dy.double(), cos, sin, at, layout, back=True)
+        within("dx", dx, value.transpose(1, 2), (half * value.abs() + 3 * U * size).transpose(1, 2))
+        assert torch.equal(y[..., R:].cpu(), x[..., R:].transpose(1, 2))
+
+
+def test_rotary_agrees_with_rope_heads():
+    """Whole heads, interleaved pairs, row t at position t: rope_heads, but for its two roundings instead of one."""
+    gen = torch.Generator(device=DEV).manual_seed(1)
+    x = torch.randn(2, 64, 4, 128, device=DEV, generator=gen, dtype=F32)
+    cos, sin = (torch.from_numpy(t.copy()).to(DEV) for t in rope.rope_tables(64, 128, 1e4))
+    torch.testing.assert_close(F.rotary_heads(x, cos, sin, layout="interleaved"), F.rope_heads(x, cos, sin),
+                               rtol=0, atol=3 * U * float(2 * x.abs().max()))
+
+
+def test_rotary_positions_outside_the_tables():
+    x = torch.ones(1, 4, 2, 64, device=DEV)
+    cos, sin = (torch.from_numpy(t).to(DEV) for t in rope.scaled_rope_tables(5, 32, 1e4))
+    at = torch.tensor([[0, 5, -1, 4]], dtype=torch.int32, device=DEV)
+    y = F.rotary_heads(x, cos, sin, positions=at)
+    assert torch.isnan(y[:, :, 1:3, :32]).all() and torch.isfinite(y[:, :, [0, 3]]).all()
+    assert (y[..., 32:] == 1).all()
+
+
+def test_rotary_of_strided_inputs_and_gradients():
+    gen = torch.Generator(device=DEV).manual_seed(4)
+    x = torch.randn(2, 30, 3, 64, device=DEV, generator=gen, dtype=BF)
+    cos, sin = (torch.from_numpy(t).to(DEV) for t in rope.scaled_rope_tables(30, 64, 1e4))
+    want = F.rotary_heads(x, cos, sin)
+    for given in (x.transpose(2, 3).contiguous().transpose(2, 3), x.transpose(0, 1).contiguous().transpose(0, 1),
+                  torch.cat([x.new_zeros(1), x.reshape(-1)])[1:].view(x.shape), torch.cat([x, x[..., :1]], 3)[..., :64]):
+        assert torch.equal(F.rotary_heads(given, cos, sin), want)
+    leaf = x.float().requires_grad_()
+    F.rotary_heads(leaf[:, :, :1].expand(2, 30, 3, 64), cos, sin).sum().backward()  # expanded input and gradient
+    value, size = turned(torch.ones(2, 3, 30, 64, dtype=torch.float64), cos.cpu(), sin.cpu(),
+                         torch.arange(30).expand(2, 30), "half", back=True)
+    within("dx", leaf.grad[:, :, :1], value.sum(1, keepdim=True).transpose(1, 2), 8 * U * size.sum(1, keepdim=True).transpose(1, 2))
+
+
+def test_rotary_refusals():
+    x = torch.zeros(1, 4, 2, 64, device=DEV)
+    c = torch.zeros(4, 32, device=DEV)
+    for call, match in (
+            (lambda: F.rotary_heads(x, c, c, layout="whole"), "layout"), (lambda: F.rotary_heads(x[0], c, c), "takes x"),
+            (lambda: F.rotary_heads(x, c[:3], c[:3]), "positions"), (lambda: F.rotary_heads(x, c, c[:, :3]), "sin must"),
+            (lambda: F.rotary_heads(x, c.half(), c.half()), "cos must"),
+            (lambda: F.rotary_heads(x, c.repeat(1, 2), c.repeat(1, 2)), "pairs"),
+            (lambda: F.rotary_heads(x, c[:, :0], c[:, :0]), "pairs"),
+            (lambda: F.rotary_heads(x, c, c, positions=torch.zeros(1, 4, device=DEV)), "positions must"),
+            (lambda: F.rotary_heads(x, c, c, positions=torch.zeros(2, 4, device=DEV, dtype=torch.int32)), "positions must"),
+            (lambda: F.rotary_heads(x, c.requires_grad_(), c.detach()), "no gradient"),
+            (lambda: F.rotary_heads(x[:0], c, c), "takes x"), (lambda: F.rotary_heads(x.half(), c, c), "not supported")):
+        with pytest.raises(ValueError, match=match):
+            call()
+        c = c.detach()
+    with pytest.raises(RuntimeError, match="ROCm"):
+        F.rotary_heads(x, c.cpu(), c)
+
+
+# ---- layer norm ---------------------------------------------------------------------------------------------------
+
+def layer_norm_ref(x, w, b, dy, eps, half):
+    """Values and first-order bounds, doubled: a mean of D terms, a square sum, one rounding of each result."""
+    x, w, dy = x.double(), w.double(), dy.double()
+    D, rows = x.shape[-1], x.numel() // x.shape[-1]
+    n = min(D, 64) + D // 64 + 16  # depth of the longest chain of additions, generously
+    mu = x.mean(-1, keepdim=True)
+    c = x - mu
+    var = (c * c).mean(-1, keepdim=True)
+    rs = 1 / torch.sqrt(var + eps)
+    xh = c * rs
+    mu_err = n * U * x.abs().mean(-1, keepdim=True)
+    rs_rel = (n + 8) * U + rs * rs * (mu_err * c.abs().mean(-1, keepdim=True) + mu_err**2)
+    xh_err = (mu_err + U * c.abs()) * rs + xh.abs() * (rs_rel + 2 * U)
+    y = xh * w + (0 if b is None else b.double())
+    out = {"y": (y, half * y.abs() + 2 * (xh_err * w.abs() + 3 * U * (xh * w).abs()))}
+    g = dy * w
+    m1, m2 = g.mean(-1, keepdim=True), (g * xh).mean(-1, keepdim=True)
+    m1_err = n * U * g.abs().mean(-1, keepdim=True)
+    m2_err = (n * U * (g * xh).abs() + g.abs() * xh_err).mean(-1, keepdim=True)
+    dx = rs * (g - m1 - xh * m2)
+    size = g.abs() + m1.abs() + (xh * m2).abs()
+    dx_err = rs * (m1_err + xh.abs() * m2_err + xh_err * m2.abs() + 6 * U * size) + rs * size * rs_rel
+    out["dx"] = (dx, half * dx.abs() + 2 * dx_err)
+    k = rows + 16
+    dw = (dy * xh).reshape(rows, D).sum(0)
+    out["dw"] = (dw, half * dw.abs() + 2 * (k * U * (dy * xh).abs() + dy.abs() * xh_err).reshape(rows, D).sum(0))
+    db = dy.reshape(rows, D).sum(0)
+    out["db"] = (db, half * db.abs() + 2 * k * U * dy.abs().reshape(rows, D).sum(0))
+    return out
+
+
+NORM = [
+    # dtype, shape, bias
+    (BF, (1, 1), True), (F32, (3, 2), True), (BF, (7, 63), True), (F32, (5, 64), False), (BF, (2, 9, 65), False),
+    (BF, (37, 2048), True), (F32, (9, 2052), True), (BF, (6, 2049), True), (F32, (5, 1000), True), (BF, (33, 128), True),
+    (BF, (4, 8192), True), (F32, (3, 5005), False), (BF, (3, 8200), True), (F32, (2, 16384), True), (BF, (3, 12001), True),
+    (F32, (2, 32768), True), (BF, (2, 40000), True), (F32, (3, 33333), True), (F32, (4111, 40), True), (BF, (2500, 520), False),
+    (F32, (700, 9000), True),
+]
+
+
+@pytest.mark.parametrize("dtype,shape,bias", NORM)
+def test_layer_norm(dtype, shape, bias):
+    gen = torch.Generator().manual_seed(shape[-1])
+    x = (torch.randn(shape, generator=gen) * 2 + 0.7).to(dtype)
+    w = (1 + 0.2 * torch.randn(shape[-1], generator=gen)).to(dtype)
+    b = torch.randn(shape[-1], generator=gen).to(dtype) if bias else None
+    dy = torch.randn(shape, generator=gen).to(dtype)
+    leaves = [t.to(DEV).requires_grad_() for t in (x, w, b) if t is not None]
+    y = F.layer_norm(*leaves[:2], leaves[2] if bias else None, 1e-5)
+    grads = torch.autograd.grad(y, leaves, dy.to(DEV))
+    ref = layer_norm_ref(x, w, b, dy, 1e-5, torch.finfo(dtype).eps / 2)
+    for name, got in zip(("y", "dx", "dw", "db"), (y, *grads)):
+        assert got.dtype == dtype
+        within(name, got, *ref[name])
+
+
+def test_layer_norm_of_constant_rows():
+    """Rows without variance: y is the bias, the gradient stays finite; the mean of one value is exact."""
+    x = torch.tensor([[3.0] * 70, [0.0] * 70, [-1e4] * 70], device=DEV, requires_grad=True)
+    w, b = torch.full((70,), 2.0, device=DEV, requires_grad=True), torch.arange(70.0, device=DEV)
+    y = F.layer_norm(x, w, b)
+    # the mean is off by at most 70 U |x|, and 1 / sqrt(eps) is 316
+    assert ((y - b).abs() <= 2 * 316 * 2 * 70 * U * x.abs()).all()
+    y.sum().backward()
+    assert torch.isfinite(x.grad).all()
+
+
+def test_layer_norm_keeps_non_finite_rows_apart():
+    gen = torch.Generator(device=DEV).manual_seed(3)
+    for D in (128, 2048, 5005, 9000):
+        x = torch.randn(9, D, device=DEV, generator=gen)
+        clean = F.layer_norm(x, torch.ones(D, device=DEV))
+        x[4, D // 2] = float("nan")
+        x[6, 0] = float("inf")
+        y = F.layer_norm(x, torch.ones(D, device=DEV))
+        assert torch.isnan(y[4]).all() and torch.isnan(y[6]).any()
+        keep = [0, 1, 2, 3, 5, 7, 8]
+        assert torch.equal(y[keep], clean[keep])
+
+
+def test_layer_norm_weight_of_another_type_and_layouts():
+    gen = torch.Generator().manual_seed(8)
+    x, dy = torch.randn(40, 96, generator=gen).to(BF), torch.randn(40, 96, generator=gen).to(BF)
+    w, b = torch.randn(96, generator=gen).to(BF).float(), torch.randn(96, generator=gen).to(BF).float()
+    ref = layer_norm_ref(x, w, b, dy, 1e-5, 2.0**-8)
+    ref["dw"], ref["db"] = (layer_norm_ref(x, w, b, dy, 1e-5, U)[n] for n in ("dw", "db"))
+    views = [x.to(DEV), x.T.contiguous().T.to(DEV), torch.cat([x.new_zeros(1), x.reshape(-1)]).to(DEV)[1:].view(40, 96),
+             torch.cat([x, x], 1).to(DEV)[:, :96]]
+    for view in views:
+        leaves = [view.detach().requires_grad_(), w.to(DEV).requires_grad_(), b.to(DEV).requires_grad_()]
+        y = F.layer_norm(*leaves)
+        grads = torch.autograd.grad(y, leaves, dy.T.contiguous().T.to(DEV))
+        assert grads[1].dtype == F32
+        for name, got in zip(("y", "dx", "dw", "db"), (y, *grads)):
+            within(name, got, *ref[name])
+
+
+def test_layer_norm_repeats_and_partial_gradients():
+    gen = torch.Generator(device=DEV).manual_seed(8)
+    x, dy = (torch.randn(3000, 1024, device=DEV, generator=gen, dtype=BF) for _ in "xy")
+    w = torch.ones(1024, device=DEV, dtype=BF, requires_grad=True)
+    runs = [torch.autograd.grad(F.layer_norm(x, w), w, dy)[0] for _ in range(2)]
+    assert torch.equal(*runs)
+    b = torch.zeros(1024, device=DEV, dtype=BF, requires_grad=True)
+    (db,) = torch.autograd.grad(F.layer_norm(x, w.detach(), b), b, dy)
+    value = dy.double().sum(0).cpu()
+    within("db", db, value, 2.0**-8 * value.abs() + 2 * 3000 * U * dy.double().abs().sum(0).cpu())
+
+
+def test_layer_norm_captured_and_replayed():
+    gen = torch.Generator(device=DEV).manual_seed(8)
+    x, dy = (torch.randn(500, 776, device=DEV, generator=gen) for _ in "xy")
+    w, b = torch.randn(776, device=DEV, generator=gen), torch.randn(776, device=DEV, generator=gen)
+    cos, sin = (torch.from_numpy(t).to(DEV) for t in rope.scaled_rope_tables(500, 8, 1e4))
+
+    def step():
+        leaves = [t.detach().requires_grad_() for t in (x, w, b)]
+        y = F.rotary_heads(F.layer_norm(*leaves).view(1, 500, 97, 8), cos, sin)
+        return [y.detach(), *torch.autograd.grad(y, leaves, dy.view(y.shape))]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for _ in range(3):
+        x.normal_(generator=gen)
+        dy.normal_(generator=gen)
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, c in zip(out, step()):
+            assert torch.equal(a, c)
+
+
+def test_layer_norm_refusals():
+    x, w = torch.zeros(4, 64, device=DEV), torch.zeros(64, device=DEV)
+    for call, match in ((lambda: F.layer_norm(x, w[:32]), "weight"), (lambda: F.layer_norm(x, w, w[:3]), "bias"),
+                        (lambda: F.layer_norm(x, w, w.bfloat16()), "beside"), (lambda: F.layer_norm(x[:0], w), "empty"),
+                        (lambda: F.layer_norm(x[:, :0], w[:0]), "empty"), (lambda: F.layer_norm(x.half(), w), "not supported"),
+                        (lambda: F.layer_norm(x, w.half()), "not supported")):
+        with pytest.raises(ValueError, match=match):
+            call()
+    with pytest.raises(RuntimeError, match="ROCm"):
+        F.layer_norm(x, w.cpu())
