@@ -26,7 +26,8 @@
 //
 // Masked pairs contribute nothing, whatever their rows hold.  A weight of 0 times a NaN or an
 // infinity is NaN, so a tile that some rows of the workgroup do not see whole is checked for
-// non-finite values as it is staged, and such a tile takes a slow path that skips zero weights.
+// non-finite values, and a workgroup that finds one does its rows over, one at a time
+// (careful_row), with products of visible pairs only.
 #include "otx_args.h"
 #include "otx_common.h"
 
@@ -48,19 +49,55 @@ constexpr int kThreads = 256;
 
 // ---- matrix products of a storage type -----------------------------------------------------
 // Rows of a tile lie in LDS with D * sizeof(T) bytes each, cut into 16-byte chunks; chunk c of
-// row r is kept at position c ^ swizzle(r).
+// row r is kept at position c ^ swizzle(r).  All of a lane's addresses in a tile are one base
+// with a constant exclusive-or and a constant offset.
 template <typename T, int D>
 struct Tile {
   static constexpr int NC = D * (int)sizeof(T) / 16;  // chunks in a row
   static constexpr int KS = NC / 2;                   // steps over D of a row product (a chunk for each half-wave)
   static constexpr int DT = D / 32;
   static constexpr int RB = D * (int)sizeof(T);
+  static constexpr int SUB = 32 * RB;  // bytes of 32 rows
 
-  static constexpr int SW = NC == 16 ? 15 : 7;
-  __device__ static __forceinline__ int swizzle(int row) { return row & SW; }
+  // A row product reads the same chunk of 16 rows at a time, and a transposing read four neighbouring
+  // chunks of four rows: both spread over all 64 banks.  (Row & 15 alone makes the transposing reads
+  // 2.3 times slower: 6.8 clocks against 3.0, measured on 8 waves that read nothing else.)  Binary32
+  // column reads take half the banks from row r and half from row r + 4.
+  static constexpr int SW = NC == 32 ? 7 : 15;  // the swizzle repeats after SW + 1 rows
+  __device__ static __forceinline__ int swizzle(int row) {
+    if constexpr (sizeof(T) == 4 && NC == 32) return (row & 3) | (row & 4) << 1;
+    if constexpr (sizeof(T) == 4) return (row & 3) | (row & 4) << 1 | (row & 8) >> 1;
+    if constexpr (NC == 16) return (row & 3) << 2 | ((row >> 2) & 3);
+    return (row & 2) << 1 | ((row >> 2) & 3);
+  }
   __device__ static __forceinline__ int at(int row, int chunk) { return row * RB + ((chunk ^ swizzle(row)) << 4); }
-  __device__ static __forceinline__ u32x4 row_frag(const char* lds, int row, int chunk) {
-    return *(const u32x4*)(lds + at(row, chunk));
+
+  // Row fragments: lane l takes row l % 32 of 32, chunks 2 ks + l / 32.
+  __device__ static __forceinline__ uint32_t row_base(uint32_t lds, int lane) { return lds + at(lane & 31, lane >> 5); }
+  // Column fragments of 32 rows: see cols().
+  __device__ static __forceinline__ uint32_t col_base(uint32_t lds, int lane) {
+    if constexpr (sizeof(T) == 2) {
+      const int col = 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+      return lds + at(4 * (lane >> 5) + ((lane & 15) >> 2), col >> 3) + (col & 7) * 2;
+    } else {
+      return lds + at(4 * (lane >> 5), (lane & 31) >> 2) + (lane & 3) * 4;
+    }
+  }
+};
+
+template <typename V>
+__device__ __forceinline__ V lds_at(uint32_t address) {
+  return *(const __attribute__((address_space(3))) V*)address;
+}
+
+// The row fragments of 32 tile rows.
+template <typename T, int D>
+struct Rows {
+  using L = Tile<T, D>;
+  u32x4 f[L::KS];
+  __device__ __forceinline__ void read(uint32_t base) {
+#pragma unroll
+    for (int ks = 0; ks < L::KS; ks++) f[ks] = lds_at<u32x4>(base ^ (ks << 5));
   }
 };
 
@@ -77,75 +114,67 @@ __device__ __forceinline__ f32x16 mma_rows(u32x4 a, u32x4 b, f32x16 c) {
   }
 }
 
-// acc[dt][d][n] += sum over the 32 tile rows k0 + 0..31 of X[k][32 dt + d] W[k][n], W in result layout.
+// The transposed fragments of 32 tile rows X[k], for acc[dt][d][n] += sum_k X[k][32 dt + d] W[k][n]
+// with W in result layout: element r of a lane in half-wave h is row otx_row(r, h).
 template <typename T, int D>
-__device__ __forceinline__ void mma_cols(f32x16 (&acc)[D / 32], const char* lds, int k0, const f32x16& w, int lane) {
-  using L = Tile<T, D>;
-  const int h = lane >> 5;
-  if constexpr (sizeof(T) == 2) {
+struct Cols;
+
+template <int D>
+struct Cols<uint16_t, D> {
+  using L = Tile<uint16_t, D>;
+  s16x4 f[2][L::DT][2];
+  // 16 lanes of a transposing read take rows k .. k + 3, columns 16 g .. 16 g + 15: lane i addresses
+  // row k + i / 4, columns 4 (i % 4) .., and receives column i of the four rows.
+  __device__ __forceinline__ void read(uint32_t base) {
+    typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+#pragma unroll
+    for (int s = 0; s < 2; s++)
+#pragma unroll
+      for (int dt = 0; dt < L::DT; dt++)
+#pragma unroll
+        for (int g = 0; g < 2; g++)
+          f[s][dt][g] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+              (lds_s16x4*)((base ^ (dt << 6 | g << 5)) + (16 * s + 8 * g) * L::RB));
+  }
+  __device__ __forceinline__ void mma(f32x16 (&acc)[L::DT], const f32x16& w) const {
 #pragma unroll
     for (int s = 0; s < 2; s++) {
       bf16x8 b;
 #pragma unroll
       for (int j = 0; j < 8; j++) b[j] = (__bf16)w[8 * s + j];
-      // 16 lanes of a transposing read take rows k .. k + 3, columns 16 g .. 16 g + 15: lane i
-      // addresses row k + i / 4, columns 4 (i % 4) .., and receives column i of the four rows
-      const int row = k0 + 16 * s + 4 * h + ((lane & 15) >> 2);
-      const int col = 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
 #pragma unroll
       for (int dt = 0; dt < L::DT; dt++) {
-        const int c = (32 * dt + col) >> 3, off = (col & 7) * 2;
-        typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
-        const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(lds + L::at(row, c) + off));
-        const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(lds + L::at(row + 8, c) + off));
-        const s16x8 a = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+        const s16x8 a = __builtin_shufflevector(f[s][dt][0], f[s][dt][1], 0, 1, 2, 3, 4, 5, 6, 7);
         acc[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), b, acc[dt], 0, 0, 0);
       }
     }
-  } else {
+  }
+};
+
+template <int D>
+struct Cols<float, D> {
+  using L = Tile<float, D>;
+  float f[16][L::DT];
+  __device__ __forceinline__ void read(uint32_t base) {
 #pragma unroll
-    for (int r = 0; r < 16; r++) {
-      const int row = k0 + otx_row(r, 0) + 4 * h;
+    for (int r = 0; r < 16; r++)
 #pragma unroll
       for (int dt = 0; dt < L::DT; dt++) {
-        const int c = 8 * dt + ((lane & 31) >> 2);
-        const float a = *(const float*)(lds + L::at(row, c) + (lane & 3) * 4);
-        acc[dt] = __builtin_amdgcn_mfma_f32_32x32x2f32(a, w[r], acc[dt], 0, 0, 0);
+        const int x = dt << 7 | L::swizzle(otx_row(r, 0)) << 4;
+        f[r][dt] = lds_at<float>((base ^ x) + otx_row(r, 0) * L::RB);
       }
-    }
   }
-}
-
-// mma_cols for a tile with non-finite values: a row of zero weight is left out.
-template <typename T, int D>
-__device__ __forceinline__ void cols_skipping(f32x16 (&acc)[D / 32], const char* lds, int k0, f32x16 w, int lane) {
-  using L = Tile<T, D>;
-  constexpr int E = 16 / (int)sizeof(T);
-#pragma unroll 1
-  for (int r = 0; r < 16; r++) {
-    const float mine = w[0];
+  __device__ __forceinline__ void mma(f32x16 (&acc)[L::DT], const f32x16& w) const {
 #pragma unroll
-    for (int i = 0; i < 15; i++) w[i] = w[i + 1];
-#pragma unroll 1
-    for (int from = 0; from < 2; from++) {
-      const float x = __shfl(mine, (lane & 31) + 32 * from);
-      int row = k0 + 8 * (r >> 2) + 4 * from + (r & 3), d0 = 4 * (lane >> 5);
-      asm("" : "+v"(row), "+v"(d0));  // addresses are formed here, not kept in registers across the kernel
+    for (int r = 0; r < 16; r++)
 #pragma unroll
       for (int dt = 0; dt < L::DT; dt++)
-#pragma unroll
-        for (int g = 0; g < 4; g++) {
-          const int d = 32 * dt + 8 * g + d0;
-          const T* p = (const T*)(lds + L::at(row, d / E)) + d % E;
-#pragma unroll
-          for (int i = 0; i < 4; i++) {
-            const float y = __builtin_fmaf(x, Elem<T>::ld(p + i), acc[dt][4 * g + i]);
-            acc[dt][4 * g + i] = x != 0.0f ? y : acc[dt][4 * g + i];
-          }
-        }
-    }
+        acc[dt] = __builtin_amdgcn_mfma_f32_32x32x2f32(f[r][dt], w[r], acc[dt], 0, 0, 0);
   }
-}
+};
+
+// Reads above it are in flight before the products below it begin.
+__device__ __forceinline__ void fence_schedule() { __builtin_amdgcn_sched_barrier(0); }
 
 template <typename T>
 __device__ __forceinline__ float element(const u32x4& v, int e) {
@@ -165,6 +194,9 @@ __device__ __forceinline__ bool nonfinite(const u32x4& v) {
   }
   return bad;
 }
+
+// For branches off the common path: registers are kept for the other side.
+__device__ __forceinline__ bool rare(bool x) { return __builtin_expect(x, 0); }
 
 // ---- which tiles take part -------------------------------------------------------------------
 struct Band {  // the mask of one batch row, apart from documents
@@ -204,7 +236,7 @@ struct TileIter {
   }
   // The next tile, or -1; `same` says whether documents and the end leave it whole.
   __device__ __forceinline__ int next(const Band& band, const i32x4* table, int nb, int lane, bool* same) {
-    while (act == 0) {
+    while (rare(act == 0)) {
       base += 64;
       if (base >= n) return -1;
       const int t = base + lane, t0 = t * BT, t1 = t0 + BT - 1;
@@ -228,34 +260,37 @@ struct TileIter {
   }
 };
 
-// Which of the pairs of one owned row and 32 rows of a tile take part: bit r for element r of a
-// result block.  The owned row is query i against keys o0 + otx_row(r, h), or key i against queries.
-template <bool OWN_QUERIES>
-__device__ __forceinline__ uint32_t visible(const Band& band, const int* lid, int o, int own, int id, int h) {
-  // relative to the first tile row of this half-wave: lo < row <= hi, or (queries own) row < pre
+// Replaces the elements of a result block whose pair does not take part.  The owned row is query
+// `own` against keys o + otx_row(r, h), or key `own` against queries.  id: what the owned row's
+// identity is, lid: those of the 32 rows.
+template <bool OWN_QUERIES, typename F>
+__device__ __forceinline__ void mask_block(const Band& band, bool same, const int* lid, int o, int own, int id, int h,
+                                           F drop) {
+  // relative to the first row of this half-wave: lo < row <= hi, or (queries own) row < pre
   const int base = o + 4 * h, w = band.window ? band.window : 0x40000000;
   const int hi = OWN_QUERIES ? own - base : own + w - 1 - base;
   const int lo = OWN_QUERIES ? own - w - base : own - 1 - base;
-  const int pre = OWN_QUERIES ? band.prefix - base : own < band.prefix ? 0x40000000 : -0x40000000;
-  uint32_t bits = 0;
+  if (band.prefix) {
+    const int pre = OWN_QUERIES ? band.prefix - base : own < band.prefix ? 0x40000000 : -0x40000000;
 #pragma unroll
-  for (int g = 0; g < 4; g++) {
-    const i32x4 ids = *(const i32x4*)(lid + 8 * g + 4 * h);
+    for (int r = 0; r < 16; r++) {
+      const int row = otx_row(r, 0);
+      drop(r, !(((row <= hi) & (row > lo)) | (row < pre)));
+    }
+  } else {
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-      const int row = 8 * g + i;
-      const bool see = (((row <= hi) & (row > lo)) | (row < pre)) & (ids[i] == id);
-      bits |= see ? 1u << (4 * g + i) : 0u;
+    for (int r = 0; r < 16; r++) drop(r, otx_row(r, 0) > hi);
+#pragma unroll
+    for (int r = 0; r < 16; r++) drop(r, otx_row(r, 0) <= lo);
+  }
+  if (!same) {
+#pragma unroll
+    for (int g = 0; g < 4; g++) {
+      const i32x4 ids = *(const i32x4*)(lid + 8 * g + 4 * h);
+#pragma unroll
+      for (int i = 0; i < 4; i++) drop(4 * g + i, ids[i] != id);
     }
   }
-  return bits;
-}
-
-// x, as a value the compiler does not know to be the same in every tile: LDS addresses formed from it
-// are computed where they are used, and do not occupy registers across the kernel.
-__device__ __forceinline__ int opaque(int x) {
-  asm volatile("" : "+v"(x));
-  return x;
 }
 
 // The identity that pairs are matched by: the document, or a value that matches nothing.
@@ -265,7 +300,19 @@ __device__ __forceinline__ int match_id(const int* doc, int i, int S, int none) 
   return d < 0 ? none : d;
 }
 
-__device__ __forceinline__ float swap_halves(float x) { return __shfl_xor(x, 32); }
+// x of this lane and of the one 32 away, joined.
+template <typename F>
+__device__ __forceinline__ float join_halves(float x, F f) {
+  typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+  const u32x2 v = __builtin_bit_cast(u32x2, __builtin_amdgcn_permlane32_swap(otx_f2u(x), otx_f2u(x), false, false));
+  return f(otx_u2f(v[0]), otx_u2f(v[1]));
+}
+__device__ __forceinline__ float sum_halves(float x) {
+  return join_halves(x, [](float a, float b) { return a + b; });
+}
+__device__ __forceinline__ float max_halves(float x) {
+  return join_halves(x, [](float a, float b) { return fmaxf(a, b); });
+}
 
 // tanh-capped score in units of log 2, from a raw dot product; for the backward t / cap is kept.
 template <typename T>
@@ -276,6 +323,23 @@ __device__ __forceinline__ float cap_tanh(float s, float sigma_over_cap) {
     const float e = __builtin_amdgcn_exp2f(s * (2.0f * kLog2e * sigma_over_cap));
     return __builtin_fmaf(-2.0f, __builtin_amdgcn_rcpf(e + 1.0f), 1.0f);
   }
+}
+
+// Copies of 16 or 4 bytes a lane straight into LDS, from base + off (off: bytes, of each lane) to lds +
+// 16 (4) * lane.  Written out so that the compiler does not count them: it cannot tell the buffer that
+// is being filled from the one that is being read, and would wait for the copies before every read of
+// LDS.  The kernels wait for them in arrived(), before the barrier that hands a buffer over.
+template <int BYTES>
+__device__ __forceinline__ void copy_lanes(const void* base, int off, uint32_t lds) {
+  if constexpr (BYTES == 16)
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(off), "s"(base)
+                 : "m0", "memory");
+  else
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2" ::"s"(lds), "v"(off), "s"(base)
+                 : "m0", "memory");
+}
+__device__ __forceinline__ uint32_t lds_address(const void* p) {
+  return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const char*)p;
 }
 
 // ---- staging -------------------------------------------------------------------------------------
@@ -295,16 +359,16 @@ struct Stage {
   }
   __device__ __forceinline__ void copy(char* lds, int row0, int S) const {
     const char* p = base + (long)row0 * stride;
-    char* to = lds + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) * 1024;
+    const uint32_t to = lds_address(lds) + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) * 1024;
     const int last = S - 1 - row0;
-    if (last >= BT - 1) {
+    if (!rare(last < BT - 1)) {
 #pragma unroll
-      for (int i = 0; i < N; i++) otx_dma16(p + (long)i * RS * stride + off, to + i * kThreads * 16);
+      for (int i = 0; i < N; i++) copy_lanes<16>(p + (long)i * RS * stride, off, to + i * kThreads * 16);
     } else {
       const int r = threadIdx.x / L::NC;
 #pragma unroll
       for (int i = 0; i < N; i++)
-        otx_dma16(p + (off + (min(r + i * RS, last) - r) * stride), to + i * kThreads * 16);
+        copy_lanes<16>(p, off + (min(r + i * RS, last) - r) * stride, to + i * kThreads * 16);
     }
   }
   // Whether this thread's share of a tile in LDS holds an infinity or a NaN.
@@ -318,7 +382,8 @@ struct Stage {
 
 // This wave's copies have arrived; with the barrier after it, everybody's.
 __device__ __forceinline__ void arrived() {
-  __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __builtin_amdgcn_s_waitcnt(0x0f70);  // the same for the compiler, which has its own loads counted as done
   __syncthreads();
 }
 
@@ -373,152 +438,6 @@ __global__ void __launch_bounds__(256) mask_table_kernel(const int* doc, i32x4* 
   }
 }
 
-// ---- forward -------------------------------------------------------------------------------------
-// Tiles are copied one ahead into the other of two buffers, with one barrier a tile.
-template <typename T, int D, bool PLAIN>
-__global__ void __launch_bounds__(kThreads, 2) mask_attn_fwd_kernel(const MaskAttnArgs a) {
-  using L = Tile<T, D>;
-  constexpr int BN = tile_rows<T>(), NT = BN / 32, BM = 128, BYTES = BN * L::RB;
-  __shared__ __align__(1024) char lk0[BYTES], lv0[BYTES], lk1[BYTES], lv1[BYTES];
-  __shared__ __align__(16) int lid[BN];
-  __shared__ int lbad;
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5;
-  const int S = a.S, nq = (S + BM - 1) / BM, nk = (S + BN - 1) / BN, nb = (S + kTab - 1) / kTab;
-  const long total = (long)a.B * a.H * nq;
-  const float cs = a.sigma * kLog2e;
-  if (threadIdx.x == 0) lbad = -1;
-  int seq = 0;  // tiles so far: lbad names the last one that held a non-finite value
-
-  for (long w = blockIdx.x; w < total; w += gridDim.x) {
-    const int bh = spread((int)(w % (a.B * a.H)), a.B * a.H), b = bh / a.H, hq = bh % a.H, hk = hq / (a.H / a.Hkv);
-    const int q0 = (nq - 1 - (int)(w / (a.B * a.H))) * BM, q1 = min(q0 + BM, S) - 1;
-    const int qw0 = q0 + 32 * wave, qw1 = min(qw0 + 31, S - 1), qi = qw0 + (lane & 31);
-    const int* doc = a.doc ? a.doc + (long)b * S : nullptr;
-    const i32x4* table = a.doc ? (const i32x4*)a.table + (long)b * nb : nullptr;
-    const Band band = {S, a.window, a.prefix ? min(max(a.prefix[b], 0), S) : 0};
-    const float slope = !PLAIN && a.slopes ? a.slopes[hq] * kLog2e : 0.0f;
-    Stage<T, D, BN> gk, gv;
-    gk.init((const T*)a.k + b * a.sk[0] + hk * a.sk[1], a.sk[2]);
-    gv.init((const T*)a.v + b * a.sv[0] + hk * a.sv[1], a.sv[2]);
-
-    TileIter<BN, true> it;
-    it.init(q0, q1, docs_of(table, q0 / kTab, q1 / kTab, nb), nk);
-    bool same = false;
-    int kb = it.next(band, table, nb, lane, &same);
-    __syncthreads();  // the last item's tiles have been read
-    if (kb >= 0) {
-      gk.copy(lk0, kb * BN, S);
-      gv.copy(lv0, kb * BN, S);
-    }
-    u32x4 qf[L::KS];
-    load_own<T, D>(qf, (const T*)a.q + b * a.sq[0] + hq * a.sq[1], a.sq[2], min(qi, S - 1), lane);
-    const int qid = match_id(doc, qi, S, -2);
-    f32x16 acc[L::DT] = {};
-    float m = -INFINITY, l = 0.0f;
-
-    auto tile = [&](const char* lk, const char* lv, char* nlk, char* nlv) {
-      const int lane = opaque(threadIdx.x & 63), h = lane >> 5;
-      const int k0 = kb * BN, k1 = k0 + BN - 1;
-      const bool cut = !same || !band.all(q0, q1, k0, k1);  // some row of the workgroup does not see it whole
-      const bool masked = !same || !band.all(qw0, qw1, k0, k1);
-      arrived();
-      kb = it.next(band, table, nb, lane, &same);
-      if (kb >= 0) {
-        gk.copy(nlk, kb * BN, S);
-        gv.copy(nlv, kb * BN, S);
-      }
-      bool bad = false;
-      if (cut) {
-        if (threadIdx.x < BN) lid[threadIdx.x] = match_id(doc, k0 + threadIdx.x, S, -1);
-        if (gv.bad(lv)) lbad = seq;
-        __syncthreads();
-        bad = lbad == seq;
-      }
-      seq++;
-      if (!band.any(qw0, qw1, k0, k1)) return;
-      f32x16 s[NT] = {};
-#pragma unroll
-      for (int t = 0; t < NT; t++)
-#pragma unroll
-        for (int ks = 0; ks < L::KS; ks++)
-          s[t] = mma_rows<T>(L::row_frag(lk, 32 * t + (lane & 31), 2 * ks + h), qf[ks], s[t]);
-      if constexpr (!PLAIN) {  // to scores in units of log 2
-        if (a.cap > 0.0f) {
-          const float soc = a.sigma / a.cap, cl = a.cap * kLog2e;
-#pragma unroll
-          for (int t = 0; t < NT; t++)
-#pragma unroll
-            for (int r = 0; r < 16; r++) s[t][r] = cl * cap_tanh<T>(s[t][r], soc);
-        } else {
-#pragma unroll
-          for (int t = 0; t < NT; t++)
-#pragma unroll
-            for (int r = 0; r < 16; r++) s[t][r] *= cs;
-        }
-        if (a.slopes) {
-#pragma unroll
-          for (int t = 0; t < NT; t++)
-#pragma unroll
-            for (int r = 0; r < 16; r++)
-              s[t][r] = __builtin_fmaf(-slope, fabsf((float)(qi - (k0 + 32 * t + otx_row(r, 0) + 4 * h))), s[t][r]);
-        }
-      }
-      if (masked) {
-#pragma unroll
-        for (int t = 0; t < NT; t++) {
-          const uint32_t see = visible<true>(band, lid + 32 * t, k0 + 32 * t, qi, qid, h);
-#pragma unroll
-          for (int r = 0; r < 16; r++) s[t][r] = (see >> r) & 1 ? s[t][r] : -INFINITY;
-        }
-      }
-      float top = s[0][0];
-#pragma unroll
-      for (int t = 0; t < NT; t++)
-#pragma unroll
-        for (int r = 0; r < 16; r++) top = fmaxf(top, s[t][r]);
-      top = fmaxf(top, swap_halves(top));
-      if constexpr (PLAIN) top *= cs;
-      // The statistics move only where a maximum grows by more than 2^8: weights stay below 2^8 and
-      // the sums, in binary32, lose nothing; most tiles then leave the accumulator as it is.
-      if (__ballot(top > m + 8.0f)) {
-        const float mn = fmaxf(m, top), f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - mn);
-        m = mn;
-        l *= f;
-#pragma unroll
-        for (int dt = 0; dt < L::DT; dt++)
-#pragma unroll
-          for (int r = 0; r < 16; r++) acc[dt][r] *= f;
-      }
-      const float mu = m == -INFINITY ? 0.0f : m;
-#pragma unroll
-      for (int t = 0; t < NT; t++) {
-#pragma unroll
-        for (int r = 0; r < 16; r++) {
-          s[t][r] = __builtin_amdgcn_exp2f(PLAIN ? __builtin_fmaf(s[t][r], cs, -mu) : s[t][r] - mu);
-          l += s[t][r];
-        }
-      }
-      if (bad) {
-#pragma unroll
-        for (int t = 0; t < NT; t++) cols_skipping<T, D>(acc, lv, 32 * t, s[t], lane);
-      } else {
-#pragma unroll
-        for (int t = 0; t < NT; t++) mma_cols<T, D>(acc, lv, 32 * t, s[t], lane);
-      }
-    };
-    while (kb >= 0) {
-      tile(lk0, lv0, lk1, lv1);
-      if (kb < 0) break;
-      tile(lk1, lv1, lk0, lv0);
-    }
-    l += swap_halves(l);
-    if (qi < S) {
-      store_own<T, D>((T*)a.out + b * a.so[0] + hq * a.so[1] + qi * a.so[2], acc, l == 0.0f ? 0.0f : 1.0f / l, lane);
-      if (h == 0) a.lse[((long)b * a.H + hq) * S + qi] = l == 0.0f ? 0.0f : m + __builtin_log2f(l);
-    }
-  }
-}
-
 // ---- backward: the weight and its gradient of one pair ------------------------------------------------
 // Element r of sv holds the raw dot product q.k, of dpv the product dO.v; on return p and dS (without sigma).
 template <typename T, bool PLAIN>
@@ -540,18 +459,283 @@ __device__ __forceinline__ void weight(const MaskAttnArgs& a, f32x16& sv, f32x16
   dpv[r] = sv[r] * (dp - dsum) * g;
 }
 
-// ---- backward: dQ, and D_i on the way ---------------------------------------------------------------
+// ---- rows next to non-finite values ------------------------------------------------------------------
+enum { kForward, kDQ, kDKDV, kDKDVPart };
+
+__device__ __forceinline__ float wave_sum(float x) {
+  for (int m = 32; m; m >>= 1) x += __shfl_xor(x, m);
+  return x;
+}
+
+template <typename T, int D>
+__device__ __forceinline__ float dot(const T* x, const T* y) {
+  float s = 0.0f;
+#pragma unroll 1
+  for (int c = 0; c < D; c += 16 / (int)sizeof(T)) {
+    const u32x4 u = *(const u32x4*)(x + c), v = *(const u32x4*)(y + c);
+#pragma unroll
+    for (int e = 0; e < Elem<T>::VEC; e++) s = __builtin_fmaf(element<T>(u, e), element<T>(v, e), s);
+  }
+  return s;
+}
+
+// One row of the result by one wave, in binary32 throughout: lanes take 64 rows of the other side for
+// the scores, then columns for the sums over those of them that the row sees, and only those.  For the
+// rows of a workgroup that met a non-finite value; slow (some 16 instructions a pair and wave).
+template <typename T, int D, int WHAT>
+__device__ __forceinline__ void careful_row(const MaskAttnArgs& a, int b, int head, int hk, int own) {
+  constexpr bool KEYS = WHAT == kDKDV || WHAT == kDKDVPart;  // the row is a key
+  constexpr int C = D / 64;
+  const int lane = threadIdx.x & 63, S = a.S;
+  const int* doc = a.doc ? a.doc + (long)b * S : nullptr;
+  const int prefix = a.prefix ? min(max(a.prefix[b], 0), S) : 0, w = a.window ? a.window : S;
+  const T* k = (const T*)a.k + b * a.sk[0] + hk * a.sk[1];
+  const T* v = (const T*)a.v + b * a.sv[0] + hk * a.sv[1];
+  float m = -INFINITY, l = 0.0f, x[C] = {}, y[C] = {};  // sums: O; dQ; dK and dV
+  const int heads = WHAT == kDKDV ? a.H / a.Hkv : 1;
+  for (int hq = head; hq < head + heads; hq++) {
+    const T* q = (const T*)a.q + b * a.sq[0] + hq * a.sq[1];
+    const T* g = (const T*)a.dout + b * a.sdo[0] + hq * a.sdo[1];
+    const long row0 = ((long)b * a.H + hq) * S;
+    const float slope = a.slopes ? a.slopes[hq] * kLog2e : 0.0f;
+    for (int base = 0; base < S; base += 64) {
+      const int other = min(base + lane, S - 1), i = KEYS ? other : own, j = KEYS ? own : other;
+      const int id = doc ? doc[own] : 0;
+      const bool see = base + lane < S && id >= 0 && (!doc || doc[other] == id) && ((j <= i && i - j < w) || j < prefix);
+      uint64_t todo = __ballot(see);
+      if (todo == 0) continue;
+      const float s = dot<T, D>(q + i * a.sq[2], k + j * a.sk[2]);
+      float u = s * (a.sigma * kLog2e), slope_of_cap = 1.0f;
+      if (a.cap > 0.0f) {
+        const float t = cap_tanh<T>(s, a.sigma / a.cap);
+        u = a.cap * kLog2e * t;
+        slope_of_cap = __builtin_fmaf(-t, t, 1.0f);
+      }
+      u = __builtin_fmaf(-slope, fabsf((float)(i - j)), u);
+      float p, ds = 0.0f;
+      if constexpr (WHAT == kForward) {
+        float top = see ? u : -INFINITY;
+        for (int x = 32; x; x >>= 1) top = fmaxf(top, __shfl_xor(top, x));
+        const float mn = fmaxf(m, top), f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - mn);
+        m = mn;
+        p = see ? __builtin_amdgcn_exp2f(u - (m == -INFINITY ? 0.0f : m)) : 0.0f;
+        l = l * f + wave_sum(p);
+#pragma unroll
+        for (int c = 0; c < C; c++) x[c] *= f;
+      } else {
+        p = __builtin_amdgcn_exp2f(u - a.lse[row0 + i]);
+        ds = p * (dot<T, D>(g + i * a.sdo[2], v + j * a.sv[2]) - a.dsum[row0 + i]) * slope_of_cap;
+      }
+      for (; todo; todo &= todo - 1) {
+        const int from = __builtin_ctzll(todo), r = base + from;
+        const float pr = __shfl(p, from), dr = __shfl(ds, from);
+#pragma unroll
+        for (int c = 0; c < C; c++) {
+          const int d = lane + 64 * c;
+          if constexpr (WHAT == kForward) {
+            x[c] = __builtin_fmaf(pr, Elem<T>::ld(v + r * a.sv[2] + d), x[c]);
+          } else if constexpr (WHAT == kDQ) {
+            x[c] = __builtin_fmaf(dr, Elem<T>::ld(k + r * a.sk[2] + d), x[c]);
+          } else {
+            x[c] = __builtin_fmaf(dr, Elem<T>::ld(q + r * a.sq[2] + d), x[c]);
+            y[c] = __builtin_fmaf(pr, Elem<T>::ld(g + r * a.sdo[2] + d), y[c]);
+          }
+        }
+      }
+    }
+  }
+  const long row = ((long)b * a.H + head) * S + own;
+#pragma unroll
+  for (int c = 0; c < C; c++) {
+    const int d = lane + 64 * c;
+    if constexpr (WHAT == kForward) {
+      ((T*)a.out)[b * a.so[0] + head * a.so[1] + own * a.so[2] + d] = Elem<T>::put(l == 0.0f ? 0.0f : x[c] / l);
+    } else if constexpr (WHAT == kDQ) {
+      ((T*)a.dq)[b * a.sdq[0] + head * a.sdq[1] + own * a.sdq[2] + d] = Elem<T>::put(x[c] * a.sigma);
+    } else if constexpr (WHAT == kDKDVPart) {
+      a.part[row * D + d] = x[c] * a.sigma;
+      a.part[(row + (long)a.B * a.H * S) * D + d] = y[c];
+    } else {
+      ((T*)a.dk)[b * a.sdk[0] + hk * a.sdk[1] + own * a.sdk[2] + d] = Elem<T>::put(x[c] * a.sigma);
+      ((T*)a.dv)[b * a.sdv[0] + hk * a.sdv[1] + own * a.sdv[2] + d] = Elem<T>::put(y[c]);
+    }
+  }
+  if (WHAT == kForward && lane == 0) a.lse[row] = l == 0.0f ? 0.0f : m + __builtin_log2f(l);
+}
+
+// ---- forward -------------------------------------------------------------------------------------
+// Tiles are copied one ahead into the other of two buffers, with one barrier a tile.
 template <typename T, int D, bool PLAIN>
-__global__ void __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) mask_attn_dq_kernel(const MaskAttnArgs a) {
+__global__ void __launch_bounds__(kThreads, 2) mask_attn_fwd_kernel(const MaskAttnArgs a) {
   using L = Tile<T, D>;
   constexpr int BN = tile_rows<T>(), NT = BN / 32, BM = 128, BYTES = BN * L::RB;
-  __shared__ __align__(1024) char lk0[BYTES], lv0[BYTES], lk1[BYTES], lv1[BYTES];
+  __shared__ __align__(1024) char lk_[2][BYTES], lv_[2][BYTES];
   __shared__ __align__(16) int lid[BN];
   __shared__ int lbad;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5;
   const int S = a.S, nq = (S + BM - 1) / BM, nk = (S + BN - 1) / BN, nb = (S + kTab - 1) / kTab;
   const long total = (long)a.B * a.H * nq;
   const float cs = a.sigma * kLog2e;
+  const uint32_t row_k = L::row_base(lds_address(lk_), lane), col_v = L::col_base(lds_address(lv_), lane);
+  if (threadIdx.x == 0) lbad = -1;
+  int seq = 0;  // tiles so far: lbad names the last one that held a non-finite value
+
+  for (long w = blockIdx.x; w < total; w += gridDim.x) {
+    const int bh = spread((int)(w % (a.B * a.H)), a.B * a.H), b = bh / a.H, hq = bh % a.H, hk = hq / (a.H / a.Hkv);
+    const int q0 = (nq - 1 - (int)(w / (a.B * a.H))) * BM, q1 = min(q0 + BM, S) - 1;
+    const int qw0 = q0 + 32 * wave, qw1 = min(qw0 + 31, S - 1), qi = qw0 + (lane & 31);
+    const int* doc = a.doc ? a.doc + (long)b * S : nullptr;
+    const i32x4* table = a.doc ? (const i32x4*)a.table + (long)b * nb : nullptr;
+    const Band band = {S, a.window, a.prefix ? min(max(a.prefix[b], 0), S) : 0};
+    const float slope = !PLAIN && a.slopes ? a.slopes[hq] * kLog2e : 0.0f;
+    Stage<T, D, BN> gk, gv;
+    gk.init((const T*)a.k + b * a.sk[0] + hk * a.sk[1], a.sk[2]);
+    gv.init((const T*)a.v + b * a.sv[0] + hk * a.sv[1], a.sv[2]);
+
+    const Docs own = docs_of(table, q0 / kTab, q1 / kTab, nb);
+    u32x4 qf[L::KS];
+    load_own<T, D>(qf, (const T*)a.q + b * a.sq[0] + hq * a.sq[1], a.sq[2], min(qi, S - 1), lane);
+    const int qid = match_id(doc, qi, S, -2);
+
+    // False, with nothing written, where a tile holds a non-finite value that some row does not see.
+    auto item = [&]() {
+      TileIter<BN, true> it;
+      it.init(q0, q1, own, nk);
+      bool same = false;
+      int kb = it.next(band, table, nb, lane, &same), buf = 0;
+      arrived();  // the last item's tiles have been read, and no copy is on its way
+      if (kb >= 0) {
+        gk.copy(lk_[buf], kb * BN, S);
+        gv.copy(lv_[buf], kb * BN, S);
+      }
+      f32x16 acc[L::DT] = {};
+      float m = -INFINITY, l = 0.0f;
+
+      auto tile = [&]() {
+        const char* lv = lv_[buf];
+        const uint32_t ak = row_k + buf * BYTES, av = col_v + buf * BYTES;
+        const int k0 = kb * BN, k1 = k0 + BN - 1;
+        const bool whole = same, cut = !same || !band.all(q0, q1, k0, k1);  // some row of the workgroup does not see it whole
+        const bool masked = !same || !band.all(qw0, qw1, k0, k1);
+        arrived();
+        kb = it.next(band, table, nb, lane, &same);
+        buf ^= 1;
+        if (kb >= 0) {
+          gk.copy(lk_[buf], kb * BN, S);
+          gv.copy(lv_[buf], kb * BN, S);
+        }
+        bool bad = false;
+        if (rare(cut)) {
+          if (threadIdx.x < BN) lid[threadIdx.x] = match_id(doc, k0 + threadIdx.x, S, -1);
+          if (gv.bad(lv)) lbad = seq;
+          __syncthreads();
+          bad = lbad == seq;
+        }
+        seq++;
+        if (rare(bad)) return false;
+        if (rare(!band.any(qw0, qw1, k0, k1))) return true;
+        f32x16 s[NT] = {};
+        Rows<T, D> kr[NT];
+        Cols<T, D> vc[NT];
+#pragma unroll
+        for (int t = 0; t < NT; t++) kr[t].read(ak + t * L::SUB);
+        fence_schedule();
+#pragma unroll
+        for (int t = 0; t < NT; t++)
+#pragma unroll
+          for (int ks = 0; ks < L::KS; ks++) s[t] = mma_rows<T>(kr[t].f[ks], qf[ks], s[t]);
+        fence_schedule();
+#pragma unroll
+        for (int t = 0; t < NT; t++) vc[t].read(av + t * L::SUB);
+        fence_schedule();
+        if constexpr (!PLAIN) {  // to scores in units of log 2
+          if (a.cap > 0.0f) {
+            const float soc = a.sigma / a.cap, cl = a.cap * kLog2e;
+#pragma unroll
+            for (int t = 0; t < NT; t++)
+#pragma unroll
+              for (int r = 0; r < 16; r++) s[t][r] = cl * cap_tanh<T>(s[t][r], soc);
+          } else {
+#pragma unroll
+            for (int t = 0; t < NT; t++)
+#pragma unroll
+              for (int r = 0; r < 16; r++) s[t][r] *= cs;
+          }
+          if (a.slopes) {
+#pragma unroll
+            for (int t = 0; t < NT; t++)
+#pragma unroll
+              for (int r = 0; r < 16; r++)
+                s[t][r] = __builtin_fmaf(-slope, fabsf((float)(qi - (k0 + 32 * t + otx_row(r, 0) + 4 * h))), s[t][r]);
+          }
+        }
+        if (rare(masked)) {
+#pragma unroll
+          for (int t = 0; t < NT; t++)
+            mask_block<true>(band, whole, lid + 32 * t, k0 + 32 * t, qi, qid, h,
+                             [&](int r, bool drop) { s[t][r] = drop ? -INFINITY : s[t][r]; });
+        }
+        float top = s[0][0];
+#pragma unroll
+        for (int t = 0; t < NT; t++)
+#pragma unroll
+          for (int r = 0; r < 16; r++) top = fmaxf(top, s[t][r]);
+        top = max_halves(top);
+        if constexpr (PLAIN) top *= cs;
+        // The statistics move only where a maximum grows by more than 2^8: weights stay below 2^8 and
+        // the sums, in binary32, lose nothing; most tiles then leave the accumulator as it is.
+        if (__ballot(top > m + 8.0f)) {
+          const float mn = fmaxf(m, top), f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - mn);
+          m = mn;
+          l *= f;
+#pragma unroll
+          for (int dt = 0; dt < L::DT; dt++)
+#pragma unroll
+            for (int r = 0; r < 16; r++) acc[dt][r] *= f;
+        }
+        const float mu = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+        for (int t = 0; t < NT; t++) {
+#pragma unroll
+          for (int r = 0; r < 16; r++) {
+            s[t][r] = __builtin_amdgcn_exp2f(PLAIN ? __builtin_fmaf(s[t][r], cs, -mu) : s[t][r] - mu);
+            l += s[t][r];
+          }
+        }
+#pragma unroll
+        for (int t = 0; t < NT; t++) vc[t].mma(acc, s[t]);
+        return true;
+      };
+      while (kb >= 0)
+        if (!tile()) return false;
+      l = sum_halves(l);
+      if (qi < S) {
+        store_own<T, D>((T*)a.out + b * a.so[0] + hq * a.so[1] + qi * a.so[2], acc, l == 0.0f ? 0.0f : 1.0f / l, lane);
+        if (h == 0) a.lse[((long)b * a.H + hq) * S + qi] = l == 0.0f ? 0.0f : m + __builtin_log2f(l);
+      }
+      return true;
+    };
+    if (rare(!item())) {
+      arrived();
+      for (int i = qw0; i <= qw1; i++) careful_row<T, D, kForward>(a, b, hq, hk, i);
+    }
+  }
+}
+
+// ---- backward: dQ, and D_i on the way ---------------------------------------------------------------
+template <typename T, int D, bool PLAIN>
+__global__ void __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) mask_attn_dq_kernel(const MaskAttnArgs a) {
+  using L = Tile<T, D>;
+  constexpr int BN = tile_rows<T>(), NT = BN / 32, BM = 128, BYTES = BN * L::RB;
+  __shared__ __align__(1024) char lk_[2][BYTES], lv_[2][BYTES];
+  __shared__ __align__(16) int lid[BN];
+  __shared__ int lbad;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5;
+  const int S = a.S, nq = (S + BM - 1) / BM, nk = (S + BN - 1) / BN, nb = (S + kTab - 1) / kTab;
+  const long total = (long)a.B * a.H * nq;
+  const float cs = a.sigma * kLog2e;
+  const uint32_t row_k = L::row_base(lds_address(lk_), lane), col_k = L::col_base(lds_address(lk_), lane);
+  const uint32_t row_v = L::row_base(lds_address(lv_), lane);
   if (threadIdx.x == 0) lbad = -1;
   int seq = 0;
 
@@ -567,15 +751,7 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) mask_attn_dq
     gk.init((const T*)a.k + b * a.sk[0] + hk * a.sk[1], a.sk[2]);
     gv.init((const T*)a.v + b * a.sv[0] + hk * a.sv[1], a.sv[2]);
 
-    TileIter<BN, true> it;
-    it.init(q0, q1, docs_of(table, q0 / kTab, q1 / kTab, nb), nk);
-    bool same = false;
-    int kb = it.next(band, table, nb, lane, &same);
-    __syncthreads();
-    if (kb >= 0) {
-      gk.copy(lk0, kb * BN, S);
-      gv.copy(lv0, kb * BN, S);
-    }
+    const Docs own = docs_of(table, q0 / kTab, q1 / kTab, nb);
     u32x4 qf[L::KS], gf[L::KS];
     load_own<T, D>(qf, (const T*)a.q + b * a.sq[0] + hq * a.sq[1], a.sq[2], qr, lane);
     load_own<T, D>(gf, (const T*)a.dout + b * a.sdo[0] + hq * a.sdo[1], a.sdo[2], qr, lane);
@@ -589,62 +765,82 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) mask_attn_dq
         for (int e = 0; e < Elem<T>::VEC; e++)
           dsum = __builtin_fmaf(element<T>(gf[ks], e), element<T>(of, e), dsum);
       }
-      dsum += swap_halves(dsum);
+      dsum = sum_halves(dsum);
     }
     const long row = ((long)b * a.H + hq) * S + qr;
     if (qi < S && h == 0) a.dsum[row] = dsum;
     const float lse = a.lse[row];
     const int qid = match_id(doc, qi, S, -2);
-    f32x16 acc[L::DT] = {};
-
-    auto tile = [&](const char* lk, const char* lv, char* nlk, char* nlv) {
-      const int lane = opaque(threadIdx.x & 63), h = lane >> 5;
-      const int k0 = kb * BN, k1 = k0 + BN - 1;
-      const bool cut = !same || !band.all(q0, q1, k0, k1);
-      const bool masked = !same || !band.all(qw0, qw1, k0, k1);
+    auto item = [&]() {
+      TileIter<BN, true> it;
+      it.init(q0, q1, own, nk);
+      bool same = false;
+      int kb = it.next(band, table, nb, lane, &same), buf = 0;
       arrived();
-      kb = it.next(band, table, nb, lane, &same);
       if (kb >= 0) {
-        gk.copy(nlk, kb * BN, S);
-        gv.copy(nlv, kb * BN, S);
+        gk.copy(lk_[buf], kb * BN, S);
+        gv.copy(lv_[buf], kb * BN, S);
       }
-      bool bad = false;
-      if (cut) {
-        if (threadIdx.x < BN) lid[threadIdx.x] = match_id(doc, k0 + threadIdx.x, S, -1);
-        if (gk.bad(lk)) lbad = seq;
-        __syncthreads();
-        bad = lbad == seq;
-      }
-      seq++;
-      if (!band.any(qw0, qw1, k0, k1)) return;
-#pragma unroll
-      for (int t = 0; t < NT; t++) {
-        f32x16 s = {}, dp = {};
-#pragma unroll
-        for (int ks = 0; ks < L::KS; ks++) {
-          s = mma_rows<T>(L::row_frag(lk, 32 * t + (lane & 31), 2 * ks + h), qf[ks], s);
-          dp = mma_rows<T>(L::row_frag(lv, 32 * t + (lane & 31), 2 * ks + h), gf[ks], dp);
+      f32x16 acc[L::DT] = {};
+
+      auto tile = [&]() {
+        const char* lk = lk_[buf];
+        const uint32_t ak = row_k + buf * BYTES, ac = col_k + buf * BYTES, av = row_v + buf * BYTES;
+        const int k0 = kb * BN, k1 = k0 + BN - 1;
+        const bool whole = same, cut = !same || !band.all(q0, q1, k0, k1);
+        const bool masked = !same || !band.all(qw0, qw1, k0, k1);
+        arrived();
+        kb = it.next(band, table, nb, lane, &same);
+        buf ^= 1;
+        if (kb >= 0) {
+          gk.copy(lk_[buf], kb * BN, S);
+          gv.copy(lv_[buf], kb * BN, S);
         }
-#pragma unroll
-        for (int r = 0; r < 16; r++)
-          weight<T, PLAIN>(a, s, dp, r, slope, cs, lse, dsum, qi - (k0 + 32 * t + 4 * h + otx_row(r, 0)));
-        if (masked) {
-          const uint32_t see = visible<true>(band, lid + 32 * t, k0 + 32 * t, qi, qid, h);
-#pragma unroll
-          for (int r = 0; r < 16; r++) dp[r] = (see >> r) & 1 ? dp[r] : 0.0f;
+        bool bad = false;
+        if (rare(cut)) {
+          if (threadIdx.x < BN) lid[threadIdx.x] = match_id(doc, k0 + threadIdx.x, S, -1);
+          if (gk.bad(lk)) lbad = seq;
+          __syncthreads();
+          bad = lbad == seq;
         }
-        if (bad)
-          cols_skipping<T, D>(acc, lk, 32 * t, dp, lane);
-        else
-          mma_cols<T, D>(acc, lk, 32 * t, dp, lane);
-      }
+        seq++;
+        if (rare(bad)) return false;
+        if (rare(!band.any(qw0, qw1, k0, k1))) return true;
+#pragma unroll
+        for (int t = 0; t < NT; t++) {
+          f32x16 s = {}, dp = {};
+          Rows<T, D> kr, vr;
+          Cols<T, D> kc;
+          kr.read(ak + t * L::SUB);
+          vr.read(av + t * L::SUB);
+          fence_schedule();
+#pragma unroll
+          for (int ks = 0; ks < L::KS; ks++) s = mma_rows<T>(kr.f[ks], qf[ks], s);
+#pragma unroll
+          for (int ks = 0; ks < L::KS; ks++) dp = mma_rows<T>(vr.f[ks], gf[ks], dp);
+          fence_schedule();
+          kc.read(ac + t * L::SUB);
+          fence_schedule();
+#pragma unroll
+          for (int r = 0; r < 16; r++)
+            weight<T, PLAIN>(a, s, dp, r, slope, cs, lse, dsum, qi - (k0 + 32 * t + 4 * h + otx_row(r, 0)));
+          if (rare(masked)) {
+            mask_block<true>(band, whole, lid + 32 * t, k0 + 32 * t, qi, qid, h,
+                             [&](int r, bool drop) { dp[r] = drop ? 0.0f : dp[r]; });
+          }
+          kc.mma(acc, dp);
+        }
+        return true;
+      };
+      while (kb >= 0)
+        if (!tile()) return false;
+      if (qi < S) store_own<T, D>((T*)a.dq + b * a.sdq[0] + hq * a.sdq[1] + qi * a.sdq[2], acc, a.sigma, lane);
+      return true;
     };
-    while (kb >= 0) {
-      tile(lk0, lv0, lk1, lv1);
-      if (kb < 0) break;
-      tile(lk1, lv1, lk0, lv0);
+    if (rare(!item())) {
+      arrived();
+      for (int i = qw0; i <= qw1; i++) careful_row<T, D, kDQ>(a, b, hq, hk, i);
     }
-    if (qi < S) store_own<T, D>((T*)a.dq + b * a.sdq[0] + hq * a.sdq[1] + qi * a.sdq[2], acc, a.sigma, lane);
   }
 }
 
@@ -655,8 +851,8 @@ template <typename T, int D, bool PLAIN, bool SPLIT>
 __global__ void __launch_bounds__(kThreads, sizeof(T) * D == 128 ? 2 : 1) mask_attn_dkdv_kernel(const MaskAttnArgs a) {
   using L = Tile<T, D>;
   constexpr int BN = tile_rows<T>(), NT = BN / 32, BM = 128, BYTES = BN * L::RB;  // BM keys owned, BN queries a tile
-  __shared__ __align__(1024) char lq0[BYTES], lg0[BYTES], lq1[BYTES], lg1[BYTES];
-  __shared__ __align__(16) float ll[2][64], ld[2][64];
+  __shared__ __align__(1024) char lq_[2][BYTES], lg_[2][BYTES];
+  __shared__ __align__(16) float ll_[2][64], ld_[2][64];
   __shared__ __align__(16) int lid[BN];
   __shared__ int lbad;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5;
@@ -664,6 +860,8 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) * D == 128 ? 2 : 1) mask_a
   const int group = a.H / a.Hkv, heads = SPLIT ? a.H : a.Hkv;
   const long total = (long)a.B * heads * nkb;
   const float cs = a.sigma * kLog2e;
+  const uint32_t row_q = L::row_base(lds_address(lq_), lane), col_q = L::col_base(lds_address(lq_), lane);
+  const uint32_t row_g = L::row_base(lds_address(lg_), lane), col_g = L::col_base(lds_address(lg_), lane);
   if (threadIdx.x == 0) lbad = -1;
   int seq = 0;
 
@@ -681,95 +879,113 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) * D == 128 ? 2 : 1) mask_a
     load_own<T, D>(kf, (const T*)a.k + b * a.sk[0] + hk * a.sk[1], a.sk[2], kr, lane);
     load_own<T, D>(vf, (const T*)a.v + b * a.sv[0] + hk * a.sv[1], a.sv[2], kr, lane);
     const int kid = match_id(doc, kj, S, -1);
-    f32x16 dk[L::DT] = {}, dv[L::DT] = {};
-
     const int first = SPLIT ? bh % heads : hk * group, last = SPLIT ? first + 1 : first + group;
-    for (int hq = first; hq < last; hq++) {
-      const long row0 = ((long)b * a.H + hq) * S;
-      const float slope = !PLAIN && a.slopes ? a.slopes[hq] * kLog2e : 0.0f;
-      Stage<T, D, BN> gq, gg;
-      gq.init((const T*)a.q + b * a.sq[0] + hq * a.sq[1], a.sq[2]);
-      gg.init((const T*)a.dout + b * a.sdo[0] + hq * a.sdo[1], a.sdo[2]);
-      TileIter<BN, false> it;
-      it.init(k0, k1, own, nq);
-      bool same = false;
-      int qb = it.next(band, table, nb, lane, &same);
-      auto stage = [&](char* lq, char* lg, int buf) {
-        gq.copy(lq, qb * BN, S);
-        gg.copy(lg, qb * BN, S);
-        const long i = row0 + min(qb * BN + lane, S - 1);  // 64 rows, BN of them read
-        if (wave == 0) otx_dma4(a.lse + i, ll[buf]);
-        if (wave == 1) otx_dma4(a.dsum + i, ld[buf]);
-      };
-      __syncthreads();
-      if (qb >= 0) stage(lq0, lg0, 0);
 
-      auto tile = [&](const char* lq, const char* lg, const int buf, char* nlq, char* nlg) {
-      const int lane = opaque(threadIdx.x & 63), h = lane >> 5;
-        const int q0 = qb * BN, q1 = q0 + BN - 1;
-        const bool cut = !same || k0 + BM > S || !band.all(q0, q1, k0, k0 + BM - 1);
-        const bool masked = !same || kw0 + 32 > S || !band.all(q0, q1, kw0, kw0 + 31);
+    auto item = [&]() {
+      f32x16 dk[L::DT] = {}, dv[L::DT] = {};
+      for (int hq = first; hq < last; hq++) {
+        const long row0 = ((long)b * a.H + hq) * S;
+        const float slope = !PLAIN && a.slopes ? a.slopes[hq] * kLog2e : 0.0f;
+        Stage<T, D, BN> gq, gg;
+        gq.init((const T*)a.q + b * a.sq[0] + hq * a.sq[1], a.sq[2]);
+        gg.init((const T*)a.dout + b * a.sdo[0] + hq * a.sdo[1], a.sdo[2]);
+        TileIter<BN, false> it;
+        it.init(k0, k1, own, nq);
+        bool same = false;
+        int qb = it.next(band, table, nb, lane, &same);
+        int buf = 0;
+        auto stage = [&]() {
+          gq.copy(lq_[buf], qb * BN, S);
+          gg.copy(lg_[buf], qb * BN, S);
+          const int i = min(qb * BN + (int)(threadIdx.x & 63), S - 1) * 4;  // 64 rows, BN of them read
+          if (wave == 0) copy_lanes<4>(a.lse + row0, i, lds_address(ll_[buf]));
+          if (wave == 1) copy_lanes<4>(a.dsum + row0, i, lds_address(ld_[buf]));
+        };
         arrived();
-        qb = it.next(band, table, nb, lane, &same);
-        if (qb >= 0) stage(nlq, nlg, 1 - buf);
-        bool bad = false;
-        if (cut) {
-          if (threadIdx.x < BN) lid[threadIdx.x] = match_id(doc, q0 + threadIdx.x, S, -2);
-          if (gq.bad(lq) || gg.bad(lg)) lbad = seq;
-          __syncthreads();
-          bad = lbad == seq;
-        }
-        seq++;
-        if (kw0 >= S || !band.any(q0, min(q1, S - 1), kw0, kw1)) return;
-#pragma unroll
-        for (int t = 0; t < NT; t++) {
-          f32x16 s = {}, dp = {};
-#pragma unroll
-          for (int ks = 0; ks < L::KS; ks++) {
-            s = mma_rows<T>(L::row_frag(lq, 32 * t + (lane & 31), 2 * ks + h), kf[ks], s);
-            dp = mma_rows<T>(L::row_frag(lg, 32 * t + (lane & 31), 2 * ks + h), vf[ks], dp);
+        if (qb >= 0) stage();
+
+        auto tile = [&]() {
+          const char *lq = lq_[buf], *lg = lg_[buf];
+          const float *ll = ll_[buf], *ld = ld_[buf];
+          const uint32_t off = buf * BYTES;
+          const int q0 = qb * BN, q1 = q0 + BN - 1;
+          const bool whole = same && kw0 + 32 <= S, cut = !same || k0 + BM > S || !band.all(q0, q1, k0, k0 + BM - 1);
+          const bool masked = !same || kw0 + 32 > S || !band.all(q0, q1, kw0, kw0 + 31);
+          arrived();
+          qb = it.next(band, table, nb, lane, &same);
+          buf ^= 1;
+          if (qb >= 0) stage();
+          bool bad = false;
+          if (rare(cut)) {
+            if (threadIdx.x < BN) lid[threadIdx.x] = match_id(doc, q0 + threadIdx.x, S, -2);
+            if (gq.bad(lq) || gg.bad(lg)) lbad = seq;
+            __syncthreads();
+            bad = lbad == seq;
           }
+          seq++;
+          if (rare(bad)) return false;
+          if (rare(kw0 >= S || !band.any(q0, min(q1, S - 1), kw0, kw1))) return true;
+          f32x16 s[NT] = {}, dp[NT] = {};
+          auto rows = [&](int t) {
+            Rows<T, D> qr, gr;
+            qr.read(row_q + off + t * L::SUB);
+            gr.read(row_g + off + t * L::SUB);
+            fence_schedule();
 #pragma unroll
-          for (int g = 0; g < 4; g++) {
-            const f32x4 x = *(const f32x4*)(ll[buf] + 32 * t + 8 * g + 4 * h);
-            const f32x4 y = *(const f32x4*)(ld[buf] + 32 * t + 8 * g + 4 * h);
-#pragma unroll
-            for (int i = 0; i < 4; i++)
-              weight<T, PLAIN>(a, s, dp, 4 * g + i, slope, cs, x[i], y[i],
-                               q0 + 32 * t + 4 * h + 8 * g + i - kj);
-          }
-          if (masked) {
-            const uint32_t see = visible<false>(band, lid + 32 * t, q0 + 32 * t, kj, kid, h);
-#pragma unroll
-            for (int r = 0; r < 16; r++) {
-              s[r] = (see >> r) & 1 ? s[r] : 0.0f;
-              dp[r] = (see >> r) & 1 ? dp[r] : 0.0f;
+            for (int ks = 0; ks < L::KS; ks++) {
+              s[t] = mma_rows<T>(qr.f[ks], kf[ks], s[t]);
+              dp[t] = mma_rows<T>(gr.f[ks], vf[ks], dp[t]);
             }
+          };
+          auto soft = [&](int t) {
+#pragma unroll
+            for (int g = 0; g < 4; g++) {
+              const f32x4 x = *(const f32x4*)(ll + 32 * t + 8 * g + 4 * h);
+              const f32x4 y = *(const f32x4*)(ld + 32 * t + 8 * g + 4 * h);
+#pragma unroll
+              for (int i = 0; i < 4; i++)
+                weight<T, PLAIN>(a, s[t], dp[t], 4 * g + i, slope, cs, x[i], y[i], q0 + 32 * t + 4 * h + 8 * g + i - kj);
+            }
+            if (rare(masked))
+              mask_block<false>(band, whole, lid + 32 * t, q0 + 32 * t, kj, kid, h, [&](int r, bool drop) {
+                s[t][r] = drop ? 0.0f : s[t][r];
+                dp[t][r] = drop ? 0.0f : dp[t][r];
+              });
+          };
+          auto cols = [&](int t) {
+            Cols<T, D> gc, qc;
+            gc.read(col_g + off + t * L::SUB);
+            qc.read(col_q + off + t * L::SUB);
+            fence_schedule();
+            gc.mma(dv, s[t]);
+            qc.mma(dk, dp[t]);
+          };
+#pragma unroll
+          for (int t = 0; t < NT; t++) {
+            rows(t);
+            soft(t);
+            cols(t);
           }
-          if (bad) {
-            cols_skipping<T, D>(dv, lg, 32 * t, s, lane);
-            cols_skipping<T, D>(dk, lq, 32 * t, dp, lane);
-          } else {
-            mma_cols<T, D>(dv, lg, 32 * t, s, lane);
-            mma_cols<T, D>(dk, lq, 32 * t, dp, lane);
-          }
+          return true;
+        };
+        while (qb >= 0)
+          if (!tile()) return false;
+      }
+      if (kj < S) {
+        if constexpr (SPLIT) {
+          float* p = a.part + (((long)b * a.H + first) * S + kj) * D;
+          store_own<float, D>(p, dk, a.sigma, lane);
+          store_own<float, D>(p + (long)a.B * a.H * S * D, dv, 1.0f, lane);
+        } else {
+          store_own<T, D>((T*)a.dk + b * a.sdk[0] + hk * a.sdk[1] + kj * a.sdk[2], dk, a.sigma, lane);
+          store_own<T, D>((T*)a.dv + b * a.sdv[0] + hk * a.sdv[1] + kj * a.sdv[2], dv, 1.0f, lane);
         }
-      };
-      while (qb >= 0) {
-        tile(lq0, lg0, 0, lq1, lg1);
-        if (qb < 0) break;
-        tile(lq1, lg1, 1, lq0, lg0);
       }
-    }
-    if (kj < S) {
-      if constexpr (SPLIT) {
-        float* p = a.part + (((long)b * a.H + first) * S + kj) * D;
-        store_own<float, D>(p, dk, a.sigma, lane);
-        store_own<float, D>(p + (long)a.B * a.H * S * D, dv, 1.0f, lane);
-      } else {
-        store_own<T, D>((T*)a.dk + b * a.sdk[0] + hk * a.sdk[1] + kj * a.sdk[2], dk, a.sigma, lane);
-        store_own<T, D>((T*)a.dv + b * a.sdv[0] + hk * a.sdv[1] + kj * a.sdv[2], dv, 1.0f, lane);
-      }
+      return true;
+    };
+    if (rare(!item())) {
+      arrived();
+      for (int j = kw0; j <= kw1; j++) careful_row<T, D, SPLIT ? kDKDVPart : kDKDV>(a, b, first, hk, j);
     }
   }
 }
