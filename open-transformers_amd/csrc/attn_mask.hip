@@ -39,6 +39,7 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef uint16_t u16x4 __attribute__((ext_vector_type(4)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef float f32x8 __attribute__((ext_vector_type(8)));
 typedef short s16x8 __attribute__((ext_vector_type(8)));
 
 namespace {
@@ -95,9 +96,10 @@ template <typename T, int D>
 struct Rows {
   using L = Tile<T, D>;
   u32x4 f[L::KS];
+  __device__ __forceinline__ void read(uint32_t base, int ks) { f[ks] = lds_at<u32x4>(base ^ (ks << 5)); }
   __device__ __forceinline__ void read(uint32_t base) {
 #pragma unroll
-    for (int ks = 0; ks < L::KS; ks++) f[ks] = lds_at<u32x4>(base ^ (ks << 5));
+    for (int ks = 0; ks < L::KS; ks++) read(base, ks);
   }
 };
 
@@ -122,31 +124,39 @@ struct Cols;
 template <int D>
 struct Cols<uint16_t, D> {
   using L = Tile<uint16_t, D>;
+  using W = bf16x8;
   s16x4 f[2][L::DT][2];
   // 16 lanes of a transposing read take rows k .. k + 3, columns 16 g .. 16 g + 15: lane i addresses
   // row k + i / 4, columns 4 (i % 4) .., and receives column i of the four rows.
-  __device__ __forceinline__ void read(uint32_t base) {
+  __device__ __forceinline__ void read(uint32_t base, int s, int dt) {
     typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+#pragma unroll
+    for (int g = 0; g < 2; g++)
+      f[s][dt][g] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+          (lds_s16x4*)((base ^ (dt << 6 | g << 5)) + (16 * s + 8 * g) * L::RB));
+  }
+  __device__ __forceinline__ void read(uint32_t base) {
 #pragma unroll
     for (int s = 0; s < 2; s++)
 #pragma unroll
-      for (int dt = 0; dt < L::DT; dt++)
+      for (int dt = 0; dt < L::DT; dt++) read(base, s, dt);
+  }
+  __device__ __forceinline__ static bf16x8 weights(const f32x16& w, int s) {
+    bf16x8 b;
 #pragma unroll
-        for (int g = 0; g < 2; g++)
-          f[s][dt][g] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-              (lds_s16x4*)((base ^ (dt << 6 | g << 5)) + (16 * s + 8 * g) * L::RB));
+    for (int j = 0; j < 8; j++) b[j] = (__bf16)w[8 * s + j];
+    return b;
+  }
+  __device__ __forceinline__ void mma(f32x16 (&acc)[L::DT], bf16x8 b, int s, int dt) const {
+    const s16x8 a = __builtin_shufflevector(f[s][dt][0], f[s][dt][1], 0, 1, 2, 3, 4, 5, 6, 7);
+    acc[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), b, acc[dt], 0, 0, 0);
   }
   __device__ __forceinline__ void mma(f32x16 (&acc)[L::DT], const f32x16& w) const {
 #pragma unroll
     for (int s = 0; s < 2; s++) {
-      bf16x8 b;
+      const bf16x8 b = weights(w, s);
 #pragma unroll
-      for (int j = 0; j < 8; j++) b[j] = (__bf16)w[8 * s + j];
-#pragma unroll
-      for (int dt = 0; dt < L::DT; dt++) {
-        const s16x8 a = __builtin_shufflevector(f[s][dt][0], f[s][dt][1], 0, 1, 2, 3, 4, 5, 6, 7);
-        acc[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), b, acc[dt], 0, 0, 0);
-      }
+      for (int dt = 0; dt < L::DT; dt++) mma(acc, b, s, dt);
     }
   }
 };
@@ -154,22 +164,41 @@ struct Cols<uint16_t, D> {
 template <int D>
 struct Cols<float, D> {
   using L = Tile<float, D>;
-  float f[16][L::DT];
+  using W = f32x8;
+  float f[2][L::DT][8];
+  __device__ __forceinline__ void read(uint32_t base, int s, int dt) {
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+      const int row = otx_row(8 * s + j, 0);
+      f[s][dt][j] = lds_at<float>((base ^ (dt << 7 | L::swizzle(row) << 4)) + row * L::RB);
+    }
+  }
   __device__ __forceinline__ void read(uint32_t base) {
 #pragma unroll
-    for (int r = 0; r < 16; r++)
+    for (int s = 0; s < 2; s++)
 #pragma unroll
-      for (int dt = 0; dt < L::DT; dt++) {
-        const int x = dt << 7 | L::swizzle(otx_row(r, 0)) << 4;
-        f[r][dt] = lds_at<float>((base ^ x) + otx_row(r, 0) * L::RB);
-      }
+      for (int dt = 0; dt < L::DT; dt++) read(base, s, dt);
+  }
+  __device__ __forceinline__ static W weights(const f32x16& w, int s) {
+    W b;
+#pragma unroll
+    for (int j = 0; j < 8; j++) b[j] = w[8 * s + j];
+    return b;
+  }
+  __device__ __forceinline__ void mma(f32x16 (&acc)[L::DT], W b, int s, int dt) const {
+#pragma unroll
+    for (int j = 0; j < 8; j++) acc[dt] = __builtin_amdgcn_mfma_f32_32x32x2f32(f[s][dt][j], b[j], acc[dt], 0, 0, 0);
   }
   __device__ __forceinline__ void mma(f32x16 (&acc)[L::DT], const f32x16& w) const {
 #pragma unroll
-    for (int r = 0; r < 16; r++)
+    for (int s = 0; s < 2; s++) {
+      const W b = weights(w, s);
 #pragma unroll
-      for (int dt = 0; dt < L::DT; dt++)
-        acc[dt] = __builtin_amdgcn_mfma_f32_32x32x2f32(f[r][dt], w[r], acc[dt], 0, 0, 0);
+      for (int j = 0; j < 8; j++)  // the accumulators in turn
+#pragma unroll
+        for (int dt = 0; dt < L::DT; dt++)
+          acc[dt] = __builtin_amdgcn_mfma_f32_32x32x2f32(f[s][dt][j], b[j], acc[dt], 0, 0, 0);
+    }
   }
 };
 
@@ -224,38 +253,46 @@ __device__ __forceinline__ Docs docs_of(const i32x4* table, int first, int last,
   return d;
 }
 
-// The tiles of BT tokens that a range of `own` tokens meets, ascending.  Lanes test 64 tiles at a time.
+// The tiles of BT tokens that a range of `own` tokens meets: first those that all of it sees whole,
+// then those that the mask cuts, each ascending, so that the loop over whole tiles holds no mask.
+// Lanes test 64 tiles at a time.
 template <int BT, bool OWN_QUERIES>
 struct TileIter {
-  uint64_t act, whole;  // whole: one document, no padding, no token past the end
-  int base, n, current;
+  uint64_t act, docs;  // docs: of the tiles at hand, those of more than one document, with padding or past the end
+  int base, n;
+  bool cut;  // the second pass
   Docs own;
   int o0, o1;
   __device__ __forceinline__ void init(int own0, int own1, const Docs& d, int ntiles) {
-    o0 = own0, o1 = own1, own = d, n = ntiles, act = 0, base = -64;
+    o0 = own0, o1 = own1, own = d, n = ntiles, act = 0, base = -64, cut = false;
   }
-  // The next tile, or -1; `same` says whether documents and the end leave it whole.
-  __device__ __forceinline__ int next(const Band& band, const i32x4* table, int nb, int lane, bool* same) {
+  // The next tile, or -1.  mixed: whether the identities of its pairs have to be compared.
+  __device__ __forceinline__ int next(const Band& band, const i32x4* table, int nb, int lane, bool* mixed) {
     while (rare(act == 0)) {
       base += 64;
-      if (base >= n) return -1;
+      if (base >= n) {
+        if (cut) return -1;
+        cut = true;
+        base = 0;
+      }
       const int t = base + lane, t0 = t * BT, t1 = t0 + BT - 1;
-      bool a = false, w = false;
+      bool a = false, all = false, d = false;
       if (t < n) {
         a = OWN_QUERIES ? band.any(o0, o1, t0, t1) : band.any(t0, t1, o0, o1);
-        w = t1 < band.S;
+        all = OWN_QUERIES ? band.all(o0, o1, t0, t1) : band.all(t0, t1, o0, o1);
+        d = t1 >= band.S || (!OWN_QUERIES && o1 >= band.S);
         if (a && table) {
-          const Docs d = docs_of(table, t0 / kTab, t1 / kTab, nb);
-          a = d.lo <= own.hi && own.lo <= d.hi;
-          w = w && d.lo == d.hi && own.lo == own.hi && !d.pad && !own.pad;
+          const Docs x = docs_of(table, t0 / kTab, t1 / kTab, nb);
+          a = x.lo <= own.hi && own.lo <= x.hi;
+          d = d || x.lo != x.hi || own.lo != own.hi || x.pad || own.pad;
         }
       }
-      act = __ballot(a);
-      whole = __ballot(w);
+      docs = __ballot(d);
+      act = __ballot(a && cut == (d || !all));
     }
     const int i = __builtin_ctzll(act);
     act &= act - 1;
-    *same = (whole >> i) & 1;
+    *mixed = (docs >> i) & 1;
     return base + i;
   }
 };
@@ -264,7 +301,7 @@ struct TileIter {
 // `own` against keys o + otx_row(r, h), or key `own` against queries.  id: what the owned row's
 // identity is, lid: those of the 32 rows.
 template <bool OWN_QUERIES, typename F>
-__device__ __forceinline__ void mask_block(const Band& band, bool same, const int* lid, int o, int own, int id, int h,
+__device__ __forceinline__ void mask_block(const Band& band, bool mixed, const int* lid, int o, int own, int id, int h,
                                            F drop) {
   // relative to the first row of this half-wave: lo < row <= hi, or (queries own) row < pre
   const int base = o + 4 * h, w = band.window ? band.window : 0x40000000;
@@ -283,7 +320,7 @@ __device__ __forceinline__ void mask_block(const Band& band, bool same, const in
 #pragma unroll
     for (int r = 0; r < 16; r++) drop(r, otx_row(r, 0) <= lo);
   }
-  if (!same) {
+  if (mixed) {
 #pragma unroll
     for (int g = 0; g < 4; g++) {
       const i32x4 ids = *(const i32x4*)(lid + 8 * g + 4 * h);
@@ -601,8 +638,9 @@ __global__ void __launch_bounds__(kThreads, 2) mask_attn_fwd_kernel(const MaskAt
     auto item = [&]() {
       TileIter<BN, true> it;
       it.init(q0, q1, own, nk);
-      bool same = false;
-      int kb = it.next(band, table, nb, lane, &same), buf = 0;
+      bool mixed = false;
+      int kb = it.next(band, table, nb, lane, &mixed), buf = 0;
+      bool bad = false;  // a tile is not finite where some row does not see it: what is formed here is not used
       arrived();  // the last item's tiles have been read, and no copy is on its way
       if (kb >= 0) {
         gk.copy(lk_[buf], kb * BN, S);
@@ -611,29 +649,26 @@ __global__ void __launch_bounds__(kThreads, 2) mask_attn_fwd_kernel(const MaskAt
       f32x16 acc[L::DT] = {};
       float m = -INFINITY, l = 0.0f;
 
-      auto tile = [&]() {
+      auto tile = [&](auto masks) {
+        constexpr bool MASKED = decltype(masks)::value;
         const char* lv = lv_[buf];
         const uint32_t ak = row_k + buf * BYTES, av = col_v + buf * BYTES;
         const int k0 = kb * BN, k1 = k0 + BN - 1;
-        const bool whole = same, cut = !same || !band.all(q0, q1, k0, k1);  // some row of the workgroup does not see it whole
-        const bool masked = !same || !band.all(qw0, qw1, k0, k1);
+        const bool ids = mixed;
         arrived();
-        kb = it.next(band, table, nb, lane, &same);
+        kb = it.next(band, table, nb, lane, &mixed);
         buf ^= 1;
         if (kb >= 0) {
           gk.copy(lk_[buf], kb * BN, S);
           gv.copy(lv_[buf], kb * BN, S);
         }
-        bool bad = false;
-        if (rare(cut)) {
+        if constexpr (MASKED) {
           if (threadIdx.x < BN) lid[threadIdx.x] = match_id(doc, k0 + threadIdx.x, S, -1);
           if (gv.bad(lv)) lbad = seq;
           __syncthreads();
-          bad = lbad == seq;
+          bad |= lbad == seq;
         }
         seq++;
-        if (rare(bad)) return false;
-        if (rare(!band.any(qw0, qw1, k0, k1))) return true;
         f32x16 s[NT] = {};
         Rows<T, D> kr[NT];
         Cols<T, D> vc[NT];
@@ -669,10 +704,10 @@ __global__ void __launch_bounds__(kThreads, 2) mask_attn_fwd_kernel(const MaskAt
                 s[t][r] = __builtin_fmaf(-slope, fabsf((float)(qi - (k0 + 32 * t + otx_row(r, 0) + 4 * h))), s[t][r]);
           }
         }
-        if (rare(masked)) {
+        if constexpr (MASKED) {
 #pragma unroll
           for (int t = 0; t < NT; t++)
-            mask_block<true>(band, whole, lid + 32 * t, k0 + 32 * t, qi, qid, h,
+            mask_block<true>(band, ids, lid + 32 * t, k0 + 32 * t, qi, qid, h,
                              [&](int r, bool drop) { s[t][r] = drop ? -INFINITY : s[t][r]; });
         }
         float top = s[0][0];
@@ -704,10 +739,10 @@ __global__ void __launch_bounds__(kThreads, 2) mask_attn_fwd_kernel(const MaskAt
         }
 #pragma unroll
         for (int t = 0; t < NT; t++) vc[t].mma(acc, s[t]);
-        return true;
       };
-      while (kb >= 0)
-        if (!tile()) return false;
+      while (kb >= 0 && !it.cut) tile(std::false_type());
+      while (kb >= 0 && !bad) tile(std::true_type());
+      if (rare(bad)) return false;
       l = sum_halves(l);
       if (qi < S) {
         store_own<T, D>((T*)a.out + b * a.so[0] + hq * a.so[1] + qi * a.so[2], acc, l == 0.0f ? 0.0f : 1.0f / l, lane);
@@ -774,8 +809,9 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) mask_attn_dq
     auto item = [&]() {
       TileIter<BN, true> it;
       it.init(q0, q1, own, nk);
-      bool same = false;
-      int kb = it.next(band, table, nb, lane, &same), buf = 0;
+      bool mixed = false;
+      int kb = it.next(band, table, nb, lane, &mixed), buf = 0;
+      bool bad = false;  // a tile is not finite where some row does not see it: what is formed here is not used
       arrived();
       if (kb >= 0) {
         gk.copy(lk_[buf], kb * BN, S);
@@ -783,29 +819,26 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) mask_attn_dq
       }
       f32x16 acc[L::DT] = {};
 
-      auto tile = [&]() {
+      auto tile = [&](auto masks) {
+        constexpr bool MASKED = decltype(masks)::value;
         const char* lk = lk_[buf];
         const uint32_t ak = row_k + buf * BYTES, ac = col_k + buf * BYTES, av = row_v + buf * BYTES;
         const int k0 = kb * BN, k1 = k0 + BN - 1;
-        const bool whole = same, cut = !same || !band.all(q0, q1, k0, k1);
-        const bool masked = !same || !band.all(qw0, qw1, k0, k1);
+        const bool ids = mixed;
         arrived();
-        kb = it.next(band, table, nb, lane, &same);
+        kb = it.next(band, table, nb, lane, &mixed);
         buf ^= 1;
         if (kb >= 0) {
           gk.copy(lk_[buf], kb * BN, S);
           gv.copy(lv_[buf], kb * BN, S);
         }
-        bool bad = false;
-        if (rare(cut)) {
+        if constexpr (MASKED) {
           if (threadIdx.x < BN) lid[threadIdx.x] = match_id(doc, k0 + threadIdx.x, S, -1);
           if (gk.bad(lk)) lbad = seq;
           __syncthreads();
-          bad = lbad == seq;
+          bad |= lbad == seq;
         }
         seq++;
-        if (rare(bad)) return false;
-        if (rare(!band.any(qw0, qw1, k0, k1))) return true;
 #pragma unroll
         for (int t = 0; t < NT; t++) {
           f32x16 s = {}, dp = {};
@@ -824,16 +857,16 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) mask_attn_dq
 #pragma unroll
           for (int r = 0; r < 16; r++)
             weight<T, PLAIN>(a, s, dp, r, slope, cs, lse, dsum, qi - (k0 + 32 * t + 4 * h + otx_row(r, 0)));
-          if (rare(masked)) {
-            mask_block<true>(band, whole, lid + 32 * t, k0 + 32 * t, qi, qid, h,
+          if constexpr (MASKED) {
+            mask_block<true>(band, ids, lid + 32 * t, k0 + 32 * t, qi, qid, h,
                              [&](int r, bool drop) { dp[r] = drop ? 0.0f : dp[r]; });
           }
           kc.mma(acc, dp);
         }
-        return true;
       };
-      while (kb >= 0)
-        if (!tile()) return false;
+      while (kb >= 0 && !it.cut) tile(std::false_type());
+      while (kb >= 0 && !bad) tile(std::true_type());
+      if (rare(bad)) return false;
       if (qi < S) store_own<T, D>((T*)a.dq + b * a.sdq[0] + hq * a.sdq[1] + qi * a.sdq[2], acc, a.sigma, lane);
       return true;
     };
@@ -851,6 +884,7 @@ template <typename T, int D, bool PLAIN, bool SPLIT>
 __global__ void __launch_bounds__(kThreads, sizeof(T) * D == 128 ? 2 : 1) mask_attn_dkdv_kernel(const MaskAttnArgs a) {
   using L = Tile<T, D>;
   constexpr int BN = tile_rows<T>(), NT = BN / 32, BM = 128, BYTES = BN * L::RB;  // BM keys owned, BN queries a tile
+  constexpr bool PIPELINED = NT == 2 && L::KS == 8 && L::DT == 4;
   __shared__ __align__(1024) char lq_[2][BYTES], lg_[2][BYTES];
   __shared__ __align__(16) float ll_[2][64], ld_[2][64];
   __shared__ __align__(16) int lid[BN];
@@ -883,7 +917,8 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) * D == 128 ? 2 : 1) mask_a
 
     auto item = [&]() {
       f32x16 dk[L::DT] = {}, dv[L::DT] = {};
-      for (int hq = first; hq < last; hq++) {
+      bool bad = false;
+      for (int hq = first; hq < last && !bad; hq++) {
         const long row0 = ((long)b * a.H + hq) * S;
         const float slope = !PLAIN && a.slopes ? a.slopes[hq] * kLog2e : 0.0f;
         Stage<T, D, BN> gq, gg;
@@ -891,8 +926,8 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) * D == 128 ? 2 : 1) mask_a
         gg.init((const T*)a.dout + b * a.sdo[0] + hq * a.sdo[1], a.sdo[2]);
         TileIter<BN, false> it;
         it.init(k0, k1, own, nq);
-        bool same = false;
-        int qb = it.next(band, table, nb, lane, &same);
+        bool mixed = false;
+        int qb = it.next(band, table, nb, lane, &mixed);
         int buf = 0;
         auto stage = [&]() {
           gq.copy(lq_[buf], qb * BN, S);
@@ -904,73 +939,114 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) * D == 128 ? 2 : 1) mask_a
         arrived();
         if (qb >= 0) stage();
 
-        auto tile = [&]() {
+        auto tile = [&](auto masks) {
+        constexpr bool MASKED = decltype(masks)::value;
           const char *lq = lq_[buf], *lg = lg_[buf];
           const float *ll = ll_[buf], *ld = ld_[buf];
           const uint32_t off = buf * BYTES;
           const int q0 = qb * BN, q1 = q0 + BN - 1;
-          const bool whole = same && kw0 + 32 <= S, cut = !same || k0 + BM > S || !band.all(q0, q1, k0, k0 + BM - 1);
-          const bool masked = !same || kw0 + 32 > S || !band.all(q0, q1, kw0, kw0 + 31);
+          const bool ids = mixed;
           arrived();
-          qb = it.next(band, table, nb, lane, &same);
+          qb = it.next(band, table, nb, lane, &mixed);
           buf ^= 1;
           if (qb >= 0) stage();
-          bool bad = false;
-          if (rare(cut)) {
+          if constexpr (MASKED) {
             if (threadIdx.x < BN) lid[threadIdx.x] = match_id(doc, q0 + threadIdx.x, S, -2);
             if (gq.bad(lq) || gg.bad(lg)) lbad = seq;
             __syncthreads();
-            bad = lbad == seq;
+            bad |= lbad == seq;
           }
           seq++;
-          if (rare(bad)) return false;
-          if (rare(kw0 >= S || !band.any(q0, min(q1, S - 1), kw0, kw1))) return true;
           f32x16 s[NT] = {}, dp[NT] = {};
-          auto rows = [&](int t) {
-            Rows<T, D> qr, gr;
-            qr.read(row_q + off + t * L::SUB);
-            gr.read(row_g + off + t * L::SUB);
-            fence_schedule();
-#pragma unroll
-            for (int ks = 0; ks < L::KS; ks++) {
-              s[t] = mma_rows<T>(qr.f[ks], kf[ks], s[t]);
-              dp[t] = mma_rows<T>(gr.f[ks], vf[ks], dp[t]);
-            }
-          };
-          auto soft = [&](int t) {
+          Rows<T, D> qr, gr;
+          Cols<T, D> gc, qc;
+          f32x4 x[4], y[4];  // lse and D_i of a block's queries
+          auto stats = [&](int t) {
 #pragma unroll
             for (int g = 0; g < 4; g++) {
-              const f32x4 x = *(const f32x4*)(ll + 32 * t + 8 * g + 4 * h);
-              const f32x4 y = *(const f32x4*)(ld + 32 * t + 8 * g + 4 * h);
-#pragma unroll
-              for (int i = 0; i < 4; i++)
-                weight<T, PLAIN>(a, s[t], dp[t], 4 * g + i, slope, cs, x[i], y[i], q0 + 32 * t + 4 * h + 8 * g + i - kj);
+              x[g] = *(const f32x4*)(ll + 32 * t + 8 * g + 4 * h);
+              y[g] = *(const f32x4*)(ld + 32 * t + 8 * g + 4 * h);
             }
-            if (rare(masked))
-              mask_block<false>(band, whole, lid + 32 * t, q0 + 32 * t, kj, kid, h, [&](int r, bool drop) {
-                s[t][r] = drop ? 0.0f : s[t][r];
-                dp[t][r] = drop ? 0.0f : dp[t][r];
-              });
           };
-          auto cols = [&](int t) {
-            Cols<T, D> gc, qc;
-            gc.read(col_g + off + t * L::SUB);
-            qc.read(col_q + off + t * L::SUB);
+          auto scores = [&](int t, int ks) {
+            s[t] = mma_rows<T>(qr.f[ks], kf[ks], s[t]);
+            dp[t] = mma_rows<T>(gr.f[ks], vf[ks], dp[t]);
+          };
+          auto soft = [&](int t, int r) {
+            weight<T, PLAIN>(a, s[t], dp[t], r, slope, cs, x[r >> 2][r & 3], y[r >> 2][r & 3],
+                             q0 + 32 * t + 4 * h + otx_row(r, 0) - kj);
+          };
+          const uint32_t rq = row_q + off, rg = row_g + off, cq = col_q + off, cg = col_g + off;
+          qr.read(rq);
+          gr.read(rg);
+          stats(0);
+          if constexpr (!MASKED && PIPELINED) {
+            // One wave per SIMD: the weights of one block are formed beside the products of the other,
+            // two elements to two products, and fragments are read where others have just been used.
             fence_schedule();
-            gc.mma(dv, s[t]);
-            qc.mma(dk, dp[t]);
-          };
 #pragma unroll
-          for (int t = 0; t < NT; t++) {
-            rows(t);
-            soft(t);
-            cols(t);
+            for (int i = 0; i < 8; i++) {
+              scores(0, i % L::KS);
+              qr.read(rq + (NT - 1) * L::SUB, i % L::KS);
+              gr.read(rg + (NT - 1) * L::SUB, i % L::KS);
+              fence_schedule();
+            }
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+              scores(NT - 1, i % L::KS);
+              gc.read(cg, i / 4 % 2, i % L::DT);
+              qc.read(cq, i / 4 % 2, i % L::DT);
+              soft(0, 2 * i);
+              soft(0, 2 * i + 1);
+              fence_schedule();
+            }
+            stats(NT - 1);
+            typename Cols<T, D>::W p[2] = {gc.weights(s[0], 0), gc.weights(s[0], 1)};
+            typename Cols<T, D>::W d[2] = {qc.weights(dp[0], 0), qc.weights(dp[0], 1)};
+            fence_schedule();
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+              gc.mma(dv, p[i / 4 % 2], i / 4 % 2, i % L::DT);
+              qc.mma(dk, d[i / 4 % 2], i / 4 % 2, i % L::DT);
+              gc.read(cg + (NT - 1) * L::SUB, i / 4 % 2, i % L::DT);
+              qc.read(cq + (NT - 1) * L::SUB, i / 4 % 2, i % L::DT);
+              soft(NT - 1, 2 * i);
+              soft(NT - 1, 2 * i + 1);
+              fence_schedule();
+            }
+            gc.mma(dv, s[NT - 1]);
+            qc.mma(dk, dp[NT - 1]);
+          } else {
+#pragma unroll
+            for (int t = 0; t < NT; t++) {
+              if (t) {
+                qr.read(rq + t * L::SUB);
+                gr.read(rg + t * L::SUB);
+                stats(t);
+              }
+              fence_schedule();
+#pragma unroll
+              for (int ks = 0; ks < L::KS; ks++) scores(t, ks);
+              fence_schedule();
+              gc.read(cg + t * L::SUB);
+              qc.read(cq + t * L::SUB);
+#pragma unroll
+              for (int r = 0; r < 16; r++) soft(t, r);
+              if constexpr (MASKED)
+                mask_block<false>(band, ids, lid + 32 * t, q0 + 32 * t, kj, kid, h, [&](int r, bool drop) {
+                  s[t][r] = drop ? 0.0f : s[t][r];
+                  dp[t][r] = drop ? 0.0f : dp[t][r];
+                });
+              fence_schedule();
+              gc.mma(dv, s[t]);
+              qc.mma(dk, dp[t]);
+            }
           }
-          return true;
         };
-        while (qb >= 0)
-          if (!tile()) return false;
+        while (qb >= 0 && !it.cut) tile(std::false_type());
+        while (qb >= 0 && !bad) tile(std::true_type());
       }
+      if (rare(bad)) return false;
       if (kj < S) {
         if constexpr (SPLIT) {
           float* p = a.part + (((long)b * a.H + first) * S + kj) * D;
