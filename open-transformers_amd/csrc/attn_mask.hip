@@ -36,8 +36,8 @@ namespace otx {
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
-typedef uint16_t u16x4 __attribute__((ext_vector_type(4)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef float f32x8 __attribute__((ext_vector_type(8)));
 typedef short s16x8 __attribute__((ext_vector_type(8)));
@@ -202,6 +202,13 @@ struct Cols<float, D> {
   }
 };
 
+// Step i of KS: the column fragments are read while row fragments are used, into the registers that those leave.
+template <typename T, int D>
+__device__ __forceinline__ void read_step(Cols<T, D>& c, uint32_t base, int i) {
+  constexpr int EACH = Tile<T, D>::KS / (2 * Tile<T, D>::DT);
+  if (i % EACH == 0) c.read(base, i / EACH / Tile<T, D>::DT, i / EACH % Tile<T, D>::DT);
+}
+
 // Reads above it are in flight before the products below it begin.
 __device__ __forceinline__ void fence_schedule() { __builtin_amdgcn_sched_barrier(0); }
 
@@ -211,18 +218,26 @@ __device__ __forceinline__ float element(const u32x4& v, int e) {
   return otx_u2f((e & 1) ? (v[e >> 1] & 0xffff0000u) : (v[e >> 1] << 16));
 }
 
-// Whether a 16-byte chunk holds an infinity or a NaN.
+// The largest magnitude seen, as bits: from which an infinity or a NaN is told.
 template <typename T>
-__device__ __forceinline__ bool nonfinite(const u32x4& v) {
-  bool bad = false;
+struct Largest {
+  typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+  uint32_t m = 0;
+  __device__ __forceinline__ void take(const u32x4& v) {
 #pragma unroll
-  for (int i = 0; i < 4; i++) {
-    const uint32_t x = v[i];
-    bad |= (x & 0x7f800000u) == 0x7f800000u;
-    if constexpr (sizeof(T) == 2) bad |= (x & 0x7f80u) == 0x7f80u;
+    for (int i = 0; i < 4; i++) {
+      if constexpr (sizeof(T) == 2)
+        m = __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, m),
+                                                                   __builtin_bit_cast(u16x2, v[i] & 0x7fff7fffu)));
+      else
+        m = __builtin_elementwise_max(m, v[i] & 0x7fffffffu);
+    }
   }
-  return bad;
-}
+  __device__ __forceinline__ bool nonfinite() const {
+    if constexpr (sizeof(T) == 2) return (m & 0xffffu) >= 0x7f80u || m >> 16 >= 0x7f80u;
+    return m >= 0x7f800000u;
+  }
+};
 
 // For branches off the common path: registers are kept for the other side.
 __device__ __forceinline__ bool rare(bool x) { return __builtin_expect(x, 0); }
@@ -253,62 +268,68 @@ __device__ __forceinline__ Docs docs_of(const i32x4* table, int first, int last,
   return d;
 }
 
-// The tiles of BT tokens that a range of `own` tokens meets: first those that all of it sees whole,
-// then those that the mask cuts, each ascending, so that the loop over whole tiles holds no mask.
-// Lanes test 64 tiles at a time.
+// The tiles of BT tokens that a range of `own` tokens meets, 64 at a time (a lane tests one): of these
+// first the ones that all of the range sees whole, then those that the mask cuts, so that the loop over
+// whole tiles holds no mask.
 template <int BT, bool OWN_QUERIES>
 struct TileIter {
-  uint64_t act, docs;  // docs: of the tiles at hand, those of more than one document, with padding or past the end
-  int base, n;
-  bool cut;  // the second pass
+  uint64_t whole, part, docs;  // docs: tiles whose pairs need not be of one document
+  uint64_t whole0, part0;
+  int base, n, o0, o1;
+  bool cut, mixed;  // of the tile that next() returned
   Docs own;
-  int o0, o1;
   __device__ __forceinline__ void init(int own0, int own1, const Docs& d, int ntiles) {
-    o0 = own0, o1 = own1, own = d, n = ntiles, act = 0, base = -64, cut = false;
+    o0 = own0, o1 = own1, own = d, n = ntiles, whole = part = 0, base = -64, cut = mixed = false;
   }
-  // The next tile, or -1.  mixed: whether the identities of its pairs have to be compared.
-  __device__ __forceinline__ int next(const Band& band, const i32x4* table, int nb, int lane, bool* mixed) {
-    while (rare(act == 0)) {
+  // Starts over for the same range.
+  __device__ __forceinline__ void again() {
+    base = n <= 64 ? 0 : -64;
+    whole = n <= 64 ? whole0 : 0;
+    part = n <= 64 ? part0 : 0;
+  }
+  __device__ __forceinline__ int next(const Band& band, const i32x4* table, int nb, int lane) {
+    while (rare((whole | part) == 0)) {
       base += 64;
-      if (base >= n) {
-        if (cut) return -1;
-        cut = true;
-        base = 0;
-      }
+      if (base >= n) return -1;
       const int t = base + lane, t0 = t * BT, t1 = t0 + BT - 1;
       bool a = false, all = false, d = false;
       if (t < n) {
         a = OWN_QUERIES ? band.any(o0, o1, t0, t1) : band.any(t0, t1, o0, o1);
-        all = OWN_QUERIES ? band.all(o0, o1, t0, t1) : band.all(t0, t1, o0, o1);
-        d = t1 >= band.S || (!OWN_QUERIES && o1 >= band.S);
+        all = OWN_QUERIES ? band.all(o0, o1, t0, t1) : band.all(t0, t1, o0, o1) && t1 < band.S;
         if (a && table) {
           const Docs x = docs_of(table, t0 / kTab, t1 / kTab, nb);
           a = x.lo <= own.hi && own.lo <= x.hi;
-          d = d || x.lo != x.hi || own.lo != own.hi || x.pad || own.pad;
+          d = x.lo != x.hi || own.lo != own.hi || x.pad || own.pad;
         }
       }
       docs = __ballot(d);
-      act = __ballot(a && cut == (d || !all));
+      whole = whole0 = __ballot(a && all && !d);
+      part = part0 = __ballot(a && (!all || d));
     }
-    const int i = __builtin_ctzll(act);
-    act &= act - 1;
-    *mixed = (docs >> i) & 1;
+    cut = whole == 0;
+    const int i = __builtin_ctzll(cut ? part : whole);
+    if (cut)
+      part &= part - 1;
+    else
+      whole &= whole - 1;
+    mixed = (docs >> i) & 1;
     return base + i;
   }
 };
 
 // Replaces the elements of a result block whose pair does not take part.  The owned row is query
-// `own` against keys o + otx_row(r, h), or key `own` against queries.  id: what the owned row's
-// identity is, lid: those of the 32 rows.
+// `own` against keys o + otx_row(r, h), or key `own` against queries.  ok: it is a token of a document;
+// id: which, lid: those of the 32 rows (padding, below 0, equals none that is ok).
 template <bool OWN_QUERIES, typename F>
-__device__ __forceinline__ void mask_block(const Band& band, bool mixed, const int* lid, int o, int own, int id, int h,
-                                           F drop) {
-  // relative to the first row of this half-wave: lo < row <= hi, or (queries own) row < pre
-  const int base = o + 4 * h, w = band.window ? band.window : 0x40000000;
-  const int hi = OWN_QUERIES ? own - base : own + w - 1 - base;
+__device__ __forceinline__ void mask_block(const Band& band, bool mixed, const int* lid, int o, int own, bool ok,
+                                           int id, int h, F drop) {
+  // relative to the first row of this half-wave: lo < row <= hi, or (a key in the prefix) row < pre
+  const int base = o + 4 * h, w = band.window ? band.window : 0x20000000, none = -0x40000000;
+  const int end = band.S - base;
+  const int hi = ok ? OWN_QUERIES ? own - base : min(own + w - base, end) - 1 : none;
   const int lo = OWN_QUERIES ? own - w - base : own - 1 - base;
   if (band.prefix) {
-    const int pre = OWN_QUERIES ? band.prefix - base : own < band.prefix ? 0x40000000 : -0x40000000;
+    const int pre = !ok ? none : OWN_QUERIES ? band.prefix - base : own < band.prefix ? end : none;
 #pragma unroll
     for (int r = 0; r < 16; r++) {
       const int row = otx_row(r, 0);
@@ -317,8 +338,10 @@ __device__ __forceinline__ void mask_block(const Band& band, bool mixed, const i
   } else {
 #pragma unroll
     for (int r = 0; r < 16; r++) drop(r, otx_row(r, 0) > hi);
+    if (!OWN_QUERIES || band.window) {
 #pragma unroll
-    for (int r = 0; r < 16; r++) drop(r, otx_row(r, 0) <= lo);
+      for (int r = 0; r < 16; r++) drop(r, otx_row(r, 0) <= lo);
+    }
   }
   if (mixed) {
 #pragma unroll
@@ -328,13 +351,6 @@ __device__ __forceinline__ void mask_block(const Band& band, bool mixed, const i
       for (int i = 0; i < 4; i++) drop(4 * g + i, ids[i] != id);
     }
   }
-}
-
-// The identity that pairs are matched by: the document, or a value that matches nothing.
-__device__ __forceinline__ int match_id(const int* doc, int i, int S, int none) {
-  if (i >= S) return none;
-  const int d = doc ? doc[i] : 0;
-  return d < 0 ? none : d;
 }
 
 // x of this lane and of the one 32 away, joined.
@@ -362,12 +378,16 @@ __device__ __forceinline__ float cap_tanh(float s, float sigma_over_cap) {
   }
 }
 
-// Copies of 16 or 4 bytes a lane straight into LDS, from base + off (off: bytes, of each lane) to lds +
+// Copies of 16 or 4 bytes a lane straight into LDS, from `from` + off (off: bytes, of each lane) to `to` +
 // 16 (4) * lane.  Written out so that the compiler does not count them: it cannot tell the buffer that
 // is being filled from the one that is being read, and would wait for the copies before every read of
 // LDS.  The kernels wait for them in arrived(), before the barrier that hands a buffer over.
 template <int BYTES>
-__device__ __forceinline__ void copy_lanes(const void* base, int off, uint32_t lds) {
+__device__ __forceinline__ void copy_lanes(const void* from, int off, uint32_t to) {
+  const uint64_t f = (uint64_t)from;  // the same in every lane, as is `to`: told to the compiler
+  const uint64_t base = (uint64_t)__builtin_amdgcn_readfirstlane((uint32_t)(f >> 32)) << 32 |
+                        (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)f);
+  const uint32_t lds = __builtin_amdgcn_readfirstlane(to);
   if constexpr (BYTES == 16)
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(off), "s"(base)
                  : "m0", "memory");
@@ -408,12 +428,11 @@ struct Stage {
         copy_lanes<16>(p, off + (min(r + i * RS, last) - r) * stride, to + i * kThreads * 16);
     }
   }
-  // Whether this thread's share of a tile in LDS holds an infinity or a NaN.
-  __device__ __forceinline__ static bool bad(const char* lds) {
-    bool b = false;
+  // This thread's share of a tile in LDS.
+  __device__ __forceinline__ static void look(const char* lds, Largest<T>& largest) {
 #pragma unroll
-    for (int i = 0; i < N; i++) b |= nonfinite<T>(*(const u32x4*)(lds + (threadIdx.x + i * kThreads) * 16));
-    return b;
+    for (int i = 0; i < N; i++) largest.take(*(const u32x4*)(lds + (threadIdx.x + i * kThreads) * 16));
+    fence_schedule();
   }
 };
 
@@ -440,10 +459,10 @@ __device__ __forceinline__ void store_own(T* row, const f32x16 (&acc)[D / 32], f
     for (int g = 0; g < 4; g++) {
       T* p = row + 32 * dt + 8 * g + 4 * (lane >> 5);
       if constexpr (sizeof(T) == 2) {
-        u16x4 o;
-        o.x = Elem<T>::put(acc[dt][4 * g] * f), o.y = Elem<T>::put(acc[dt][4 * g + 1] * f);
-        o.z = Elem<T>::put(acc[dt][4 * g + 2] * f), o.w = Elem<T>::put(acc[dt][4 * g + 3] * f);
-        *(u16x4*)p = o;
+        bf16x4 o;
+#pragma unroll
+        for (int i = 0; i < 4; i++) o[i] = (__bf16)(acc[dt][4 * g + i] * f);
+        *(bf16x4*)p = o;
       } else {
         *(float4*)p = make_float4(acc[dt][4 * g] * f, acc[dt][4 * g + 1] * f, acc[dt][4 * g + 2] * f,
                                   acc[dt][4 * g + 3] * f);
@@ -600,6 +619,14 @@ __device__ __forceinline__ void careful_row(const MaskAttnArgs& a, int b, int he
   if (WHAT == kForward && lane == 0) a.lse[row] = l == 0.0f ? 0.0f : m + __builtin_log2f(l);
 }
 
+// Whether some thread of the workgroup met a non-finite value in the item `seq`.
+template <typename T>
+__device__ __forceinline__ bool met_nonfinite(const Largest<T>& largest, int& lbad, int seq) {
+  if (largest.nonfinite()) lbad = seq;
+  __syncthreads();
+  return lbad == seq;
+}
+
 // ---- forward -------------------------------------------------------------------------------------
 // Tiles are copied one ahead into the other of two buffers, with one barrier a tile.
 template <typename T, int D, bool PLAIN>
@@ -607,7 +634,7 @@ __global__ void __launch_bounds__(kThreads, 2) mask_attn_fwd_kernel(const MaskAt
   using L = Tile<T, D>;
   constexpr int BN = tile_rows<T>(), NT = BN / 32, BM = 128, BYTES = BN * L::RB;
   __shared__ __align__(1024) char lk_[2][BYTES], lv_[2][BYTES];
-  __shared__ __align__(16) int lid[BN];
+  __shared__ __align__(16) int lid_[2][64];
   __shared__ int lbad;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5;
   const int S = a.S, nq = (S + BM - 1) / BM, nk = (S + BN - 1) / BN, nb = (S + kTab - 1) / kTab;
@@ -615,7 +642,7 @@ __global__ void __launch_bounds__(kThreads, 2) mask_attn_fwd_kernel(const MaskAt
   const float cs = a.sigma * kLog2e;
   const uint32_t row_k = L::row_base(lds_address(lk_), lane), col_v = L::col_base(lds_address(lv_), lane);
   if (threadIdx.x == 0) lbad = -1;
-  int seq = 0;  // tiles so far: lbad names the last one that held a non-finite value
+  int seq = 0;  // items so far: lbad names the last one that met a non-finite value
 
   for (long w = blockIdx.x; w < total; w += gridDim.x) {
     const int bh = spread((int)(w % (a.B * a.H)), a.B * a.H), b = bh / a.H, hq = bh % a.H, hk = hq / (a.H / a.Hkv);
@@ -632,57 +659,51 @@ __global__ void __launch_bounds__(kThreads, 2) mask_attn_fwd_kernel(const MaskAt
     const Docs own = docs_of(table, q0 / kTab, q1 / kTab, nb);
     u32x4 qf[L::KS];
     load_own<T, D>(qf, (const T*)a.q + b * a.sq[0] + hq * a.sq[1], a.sq[2], min(qi, S - 1), lane);
-    const int qid = match_id(doc, qi, S, -2);
+    const int qid = doc ? doc[min(qi, S - 1)] : 0;
 
     // False, with nothing written, where a tile holds a non-finite value that some row does not see.
     auto item = [&]() {
       TileIter<BN, true> it;
       it.init(q0, q1, own, nk);
-      bool mixed = false;
-      int kb = it.next(band, table, nb, lane, &mixed), buf = 0;
-      bool bad = false;  // a tile is not finite where some row does not see it: what is formed here is not used
-      arrived();  // the last item's tiles have been read, and no copy is on its way
-      if (kb >= 0) {
+      int kb = it.next(band, table, nb, lane), buf = 0;
+      Largest<T> largest;  // of cut tiles: with an infinity among them, what is formed here is not used
+      auto stage = [&]() {
         gk.copy(lk_[buf], kb * BN, S);
         gv.copy(lv_[buf], kb * BN, S);
-      }
+        if (doc && wave == 0) copy_lanes<4>(doc, min(kb * BN + lane, S - 1) * 4, lds_address(lid_[buf]));
+      };
+      arrived();  // the last item's tiles have been read, and no copy is on its way
+      if (kb >= 0) stage();
       f32x16 acc[L::DT] = {};
       float m = -INFINITY, l = 0.0f;
 
-      auto tile = [&](auto masks) {
-        constexpr bool MASKED = decltype(masks)::value;
+      auto tile = [&]() {
         const char* lv = lv_[buf];
         const uint32_t ak = row_k + buf * BYTES, av = col_v + buf * BYTES;
         const int k0 = kb * BN, k1 = k0 + BN - 1;
-        const bool ids = mixed;
+        const bool cut = it.cut, ids = it.mixed;
+        const int* lid = lid_[buf];
         arrived();
-        kb = it.next(band, table, nb, lane, &mixed);
+        kb = it.next(band, table, nb, lane);
         buf ^= 1;
-        if (kb >= 0) {
-          gk.copy(lk_[buf], kb * BN, S);
-          gv.copy(lv_[buf], kb * BN, S);
-        }
-        if constexpr (MASKED) {
-          if (threadIdx.x < BN) lid[threadIdx.x] = match_id(doc, k0 + threadIdx.x, S, -1);
-          if (gv.bad(lv)) lbad = seq;
-          __syncthreads();
-          bad |= lbad == seq;
-        }
-        seq++;
+        if (kb >= 0) stage();
+        if (rare(cut)) gv.look(lv, largest);
         f32x16 s[NT] = {};
-        Rows<T, D> kr[NT];
-        Cols<T, D> vc[NT];
-#pragma unroll
-        for (int t = 0; t < NT; t++) kr[t].read(ak + t * L::SUB);
+        Rows<T, D> kr;
+        Cols<T, D> vc;
+        kr.read(ak);
         fence_schedule();
 #pragma unroll
         for (int t = 0; t < NT; t++)
 #pragma unroll
-          for (int ks = 0; ks < L::KS; ks++) s[t] = mma_rows<T>(kr[t].f[ks], qf[ks], s[t]);
-        fence_schedule();
-#pragma unroll
-        for (int t = 0; t < NT; t++) vc[t].read(av + t * L::SUB);
-        fence_schedule();
+          for (int ks = 0; ks < L::KS; ks++) {
+            s[t] = mma_rows<T>(kr.f[ks], qf[ks], s[t]);
+            if (t + 1 < NT)
+              kr.read(ak + (t + 1) * L::SUB, ks);
+            else
+              read_step(vc, av, ks);
+            fence_schedule();
+          }
         if constexpr (!PLAIN) {  // to scores in units of log 2
           if (a.cap > 0.0f) {
             const float soc = a.sigma / a.cap, cl = a.cap * kLog2e;
@@ -704,10 +725,10 @@ __global__ void __launch_bounds__(kThreads, 2) mask_attn_fwd_kernel(const MaskAt
                 s[t][r] = __builtin_fmaf(-slope, fabsf((float)(qi - (k0 + 32 * t + otx_row(r, 0) + 4 * h))), s[t][r]);
           }
         }
-        if constexpr (MASKED) {
+        if (rare(cut)) {
 #pragma unroll
           for (int t = 0; t < NT; t++)
-            mask_block<true>(band, ids, lid + 32 * t, k0 + 32 * t, qi, qid, h,
+            mask_block<true>(band, ids, lid + 32 * t, k0 + 32 * t, qi, qid >= 0, qid, h,
                              [&](int r, bool drop) { s[t][r] = drop ? -INFINITY : s[t][r]; });
         }
         float top = s[0][0];
@@ -738,11 +759,26 @@ __global__ void __launch_bounds__(kThreads, 2) mask_attn_fwd_kernel(const MaskAt
           }
         }
 #pragma unroll
-        for (int t = 0; t < NT; t++) vc[t].mma(acc, s[t]);
+        for (int t = 0; t < NT; t++) {
+          if (t + 1 < NT) {
+            fence_schedule();
+#pragma unroll
+            for (int half = 0; half < 2; half++) {
+              const auto b = vc.weights(s[t], half);
+#pragma unroll
+              for (int dt = 0; dt < L::DT; dt++) {
+                vc.mma(acc, b, half, dt);
+                vc.read(av + (t + 1) * L::SUB, half, dt);
+                fence_schedule();
+              }
+            }
+          } else {
+            vc.mma(acc, s[t]);
+          }
+        }
       };
-      while (kb >= 0 && !it.cut) tile(std::false_type());
-      while (kb >= 0 && !bad) tile(std::true_type());
-      if (rare(bad)) return false;
+      while (kb >= 0) tile();
+      if (rare(met_nonfinite(largest, lbad, seq++))) return false;
       l = sum_halves(l);
       if (qi < S) {
         store_own<T, D>((T*)a.out + b * a.so[0] + hq * a.so[1] + qi * a.so[2], acc, l == 0.0f ? 0.0f : 1.0f / l, lane);
@@ -763,7 +799,7 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) mask_attn_dq
   using L = Tile<T, D>;
   constexpr int BN = tile_rows<T>(), NT = BN / 32, BM = 128, BYTES = BN * L::RB;
   __shared__ __align__(1024) char lk_[2][BYTES], lv_[2][BYTES];
-  __shared__ __align__(16) int lid[BN];
+  __shared__ __align__(16) int lid_[2][64];
   __shared__ int lbad;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5;
   const int S = a.S, nq = (S + BM - 1) / BM, nk = (S + BN - 1) / BN, nb = (S + kTab - 1) / kTab;
@@ -805,68 +841,63 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) mask_attn_dq
     const long row = ((long)b * a.H + hq) * S + qr;
     if (qi < S && h == 0) a.dsum[row] = dsum;
     const float lse = a.lse[row];
-    const int qid = match_id(doc, qi, S, -2);
+    const int qid = doc ? doc[min(qi, S - 1)] : 0;
     auto item = [&]() {
       TileIter<BN, true> it;
       it.init(q0, q1, own, nk);
-      bool mixed = false;
-      int kb = it.next(band, table, nb, lane, &mixed), buf = 0;
-      bool bad = false;  // a tile is not finite where some row does not see it: what is formed here is not used
-      arrived();
-      if (kb >= 0) {
+      int kb = it.next(band, table, nb, lane), buf = 0;
+      Largest<T> largest;  // of cut tiles: with an infinity among them, what is formed here is not used
+      auto stage = [&]() {
         gk.copy(lk_[buf], kb * BN, S);
         gv.copy(lv_[buf], kb * BN, S);
-      }
+        if (doc && wave == 0) copy_lanes<4>(doc, min(kb * BN + lane, S - 1) * 4, lds_address(lid_[buf]));
+      };
+      arrived();
+      if (kb >= 0) stage();
       f32x16 acc[L::DT] = {};
 
-      auto tile = [&](auto masks) {
-        constexpr bool MASKED = decltype(masks)::value;
+      auto tile = [&]() {
         const char* lk = lk_[buf];
         const uint32_t ak = row_k + buf * BYTES, ac = col_k + buf * BYTES, av = row_v + buf * BYTES;
         const int k0 = kb * BN, k1 = k0 + BN - 1;
-        const bool ids = mixed;
+        const bool cut = it.cut, ids = it.mixed;
+        const int* lid = lid_[buf];
         arrived();
-        kb = it.next(band, table, nb, lane, &mixed);
+        kb = it.next(band, table, nb, lane);
         buf ^= 1;
-        if (kb >= 0) {
-          gk.copy(lk_[buf], kb * BN, S);
-          gv.copy(lv_[buf], kb * BN, S);
-        }
-        if constexpr (MASKED) {
-          if (threadIdx.x < BN) lid[threadIdx.x] = match_id(doc, k0 + threadIdx.x, S, -1);
-          if (gk.bad(lk)) lbad = seq;
-          __syncthreads();
-          bad |= lbad == seq;
-        }
-        seq++;
+        if (kb >= 0) stage();
+        if (rare(cut)) gk.look(lk, largest);
 #pragma unroll
         for (int t = 0; t < NT; t++) {
           f32x16 s = {}, dp = {};
           Rows<T, D> kr, vr;
           Cols<T, D> kc;
           kr.read(ak + t * L::SUB);
-          vr.read(av + t * L::SUB);
           fence_schedule();
 #pragma unroll
-          for (int ks = 0; ks < L::KS; ks++) s = mma_rows<T>(kr.f[ks], qf[ks], s);
-#pragma unroll
-          for (int ks = 0; ks < L::KS; ks++) dp = mma_rows<T>(vr.f[ks], gf[ks], dp);
+          for (int ks = 0; ks < L::KS; ks++) {
+            s = mma_rows<T>(kr.f[ks], qf[ks], s);
+            vr.read(av + t * L::SUB, ks);
+          }
           fence_schedule();
-          kc.read(ac + t * L::SUB);
+#pragma unroll
+          for (int ks = 0; ks < L::KS; ks++) {
+            dp = mma_rows<T>(vr.f[ks], gf[ks], dp);
+            read_step(kc, ac + t * L::SUB, ks);
+          }
           fence_schedule();
 #pragma unroll
           for (int r = 0; r < 16; r++)
             weight<T, PLAIN>(a, s, dp, r, slope, cs, lse, dsum, qi - (k0 + 32 * t + 4 * h + otx_row(r, 0)));
-          if constexpr (MASKED) {
-            mask_block<true>(band, ids, lid + 32 * t, k0 + 32 * t, qi, qid, h,
+          if (rare(cut)) {
+            mask_block<true>(band, ids, lid + 32 * t, k0 + 32 * t, qi, qid >= 0, qid, h,
                              [&](int r, bool drop) { dp[r] = drop ? 0.0f : dp[r]; });
           }
           kc.mma(acc, dp);
         }
       };
-      while (kb >= 0 && !it.cut) tile(std::false_type());
-      while (kb >= 0 && !bad) tile(std::true_type());
-      if (rare(bad)) return false;
+      while (kb >= 0) tile();
+      if (rare(met_nonfinite(largest, lbad, seq++))) return false;
       if (qi < S) store_own<T, D>((T*)a.dq + b * a.sdq[0] + hq * a.sdq[1] + qi * a.sdq[2], acc, a.sigma, lane);
       return true;
     };
@@ -887,7 +918,7 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) * D == 128 ? 2 : 1) mask_a
   constexpr bool PIPELINED = NT == 2 && L::KS == 8 && L::DT == 4;
   __shared__ __align__(1024) char lq_[2][BYTES], lg_[2][BYTES];
   __shared__ __align__(16) float ll_[2][64], ld_[2][64];
-  __shared__ __align__(16) int lid[BN];
+  __shared__ __align__(16) int lid_[2][64];
   __shared__ int lbad;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5;
   const int S = a.S, nkb = (S + BM - 1) / BM, nq = (S + BN - 1) / BN, nb = (S + kTab - 1) / kTab;
@@ -912,141 +943,151 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) * D == 128 ? 2 : 1) mask_a
     u32x4 kf[L::KS], vf[L::KS];
     load_own<T, D>(kf, (const T*)a.k + b * a.sk[0] + hk * a.sk[1], a.sk[2], kr, lane);
     load_own<T, D>(vf, (const T*)a.v + b * a.sv[0] + hk * a.sv[1], a.sv[2], kr, lane);
-    const int kid = match_id(doc, kj, S, -1);
+    const int kid = doc ? doc[kr] : 0;
     const int first = SPLIT ? bh % heads : hk * group, last = SPLIT ? first + 1 : first + group;
 
     auto item = [&]() {
       f32x16 dk[L::DT] = {}, dv[L::DT] = {};
-      bool bad = false;
-      for (int hq = first; hq < last && !bad; hq++) {
-        const long row0 = ((long)b * a.H + hq) * S;
-        const float slope = !PLAIN && a.slopes ? a.slopes[hq] * kLog2e : 0.0f;
-        Stage<T, D, BN> gq, gg;
+      Largest<T> largest;
+      int hq = first, buf = 0;  // the head whose queries are copied next
+      Stage<T, D, BN> gq, gg;
+      auto take_head = [&]() {
         gq.init((const T*)a.q + b * a.sq[0] + hq * a.sq[1], a.sq[2]);
         gg.init((const T*)a.dout + b * a.sdo[0] + hq * a.sdo[1], a.sdo[2]);
-        TileIter<BN, false> it;
-        it.init(k0, k1, own, nq);
-        bool mixed = false;
-        int qb = it.next(band, table, nb, lane, &mixed);
-        int buf = 0;
-        auto stage = [&]() {
-          gq.copy(lq_[buf], qb * BN, S);
-          gg.copy(lg_[buf], qb * BN, S);
-          const int i = min(qb * BN + (int)(threadIdx.x & 63), S - 1) * 4;  // 64 rows, BN of them read
-          if (wave == 0) copy_lanes<4>(a.lse + row0, i, lds_address(ll_[buf]));
-          if (wave == 1) copy_lanes<4>(a.dsum + row0, i, lds_address(ld_[buf]));
-        };
-        arrived();
-        if (qb >= 0) stage();
+      };
+      TileIter<BN, false> it;
+      it.init(k0, k1, own, nq);
+      int qb = it.next(band, table, nb, lane);
+      auto stage = [&]() {
+        gq.copy(lq_[buf], qb * BN, S);
+        gg.copy(lg_[buf], qb * BN, S);
+        const int i = min(qb * BN + lane, S - 1) * 4;  // 64 rows, BN of them read
+        const long row0 = ((long)b * a.H + hq) * S;
+        if (wave == 0) copy_lanes<4>(a.lse + row0, i, lds_address(ll_[buf]));
+        if (wave == 1) copy_lanes<4>(a.dsum + row0, i, lds_address(ld_[buf]));
+        if (doc && wave == 2) copy_lanes<4>(doc, i, lds_address(lid_[buf]));
+      };
+      arrived();
+      take_head();
+      if (qb >= 0) stage();
 
-        auto tile = [&](auto masks) {
-        constexpr bool MASKED = decltype(masks)::value;
-          const char *lq = lq_[buf], *lg = lg_[buf];
-          const float *ll = ll_[buf], *ld = ld_[buf];
-          const uint32_t off = buf * BYTES;
-          const int q0 = qb * BN, q1 = q0 + BN - 1;
-          const bool ids = mixed;
-          arrived();
-          qb = it.next(band, table, nb, lane, &mixed);
-          buf ^= 1;
-          if (qb >= 0) stage();
-          if constexpr (MASKED) {
-            if (threadIdx.x < BN) lid[threadIdx.x] = match_id(doc, q0 + threadIdx.x, S, -2);
-            if (gq.bad(lq) || gg.bad(lg)) lbad = seq;
-            __syncthreads();
-            bad |= lbad == seq;
-          }
-          seq++;
-          f32x16 s[NT] = {}, dp[NT] = {};
-          Rows<T, D> qr, gr;
-          Cols<T, D> gc, qc;
-          f32x4 x[4], y[4];  // lse and D_i of a block's queries
-          auto stats = [&](int t) {
+      auto tile = [&](auto masks) {
+      constexpr bool MASKED = decltype(masks)::value;
+        const char *lq = lq_[buf], *lg = lg_[buf];
+        const float *ll = ll_[buf], *ld = ld_[buf];
+        const uint32_t off = buf * BYTES;
+        const int q0 = qb * BN, q1 = q0 + BN - 1;
+        const bool cut = it.cut, ids = it.mixed;
+        const int* lid = lid_[buf];
+        const float slope = !PLAIN && a.slopes ? a.slopes[hq] * kLog2e : 0.0f;
+        arrived();
+        qb = it.next(band, table, nb, lane);
+        if (qb < 0 && hq + 1 < last) {
+          hq++;
+          take_head();
+          it.again();
+          qb = it.next(band, table, nb, lane);
+        }
+        buf ^= 1;
+        if (qb >= 0) stage();
+        if (MASKED && rare(cut)) {
+          gq.look(lq, largest);
+          gg.look(lg, largest);
+        }
+        f32x16 s[NT] = {}, dp[NT] = {};
+        Rows<T, D> qr, gr;
+        Cols<T, D> gc, qc;
+        f32x4 x[4], y[4];  // lse and D_i of a block's queries
+        auto stats = [&](int t) {
 #pragma unroll
-            for (int g = 0; g < 4; g++) {
-              x[g] = *(const f32x4*)(ll + 32 * t + 8 * g + 4 * h);
-              y[g] = *(const f32x4*)(ld + 32 * t + 8 * g + 4 * h);
-            }
-          };
-          auto scores = [&](int t, int ks) {
-            s[t] = mma_rows<T>(qr.f[ks], kf[ks], s[t]);
-            dp[t] = mma_rows<T>(gr.f[ks], vf[ks], dp[t]);
-          };
-          auto soft = [&](int t, int r) {
-            weight<T, PLAIN>(a, s[t], dp[t], r, slope, cs, x[r >> 2][r & 3], y[r >> 2][r & 3],
-                             q0 + 32 * t + 4 * h + otx_row(r, 0) - kj);
-          };
-          const uint32_t rq = row_q + off, rg = row_g + off, cq = col_q + off, cg = col_g + off;
-          qr.read(rq);
-          gr.read(rg);
-          stats(0);
-          if constexpr (!MASKED && PIPELINED) {
-            // One wave per SIMD: the weights of one block are formed beside the products of the other,
-            // two elements to two products, and fragments are read where others have just been used.
-            fence_schedule();
-#pragma unroll
-            for (int i = 0; i < 8; i++) {
-              scores(0, i % L::KS);
-              qr.read(rq + (NT - 1) * L::SUB, i % L::KS);
-              gr.read(rg + (NT - 1) * L::SUB, i % L::KS);
-              fence_schedule();
-            }
-#pragma unroll
-            for (int i = 0; i < 8; i++) {
-              scores(NT - 1, i % L::KS);
-              gc.read(cg, i / 4 % 2, i % L::DT);
-              qc.read(cq, i / 4 % 2, i % L::DT);
-              soft(0, 2 * i);
-              soft(0, 2 * i + 1);
-              fence_schedule();
-            }
-            stats(NT - 1);
-            typename Cols<T, D>::W p[2] = {gc.weights(s[0], 0), gc.weights(s[0], 1)};
-            typename Cols<T, D>::W d[2] = {qc.weights(dp[0], 0), qc.weights(dp[0], 1)};
-            fence_schedule();
-#pragma unroll
-            for (int i = 0; i < 8; i++) {
-              gc.mma(dv, p[i / 4 % 2], i / 4 % 2, i % L::DT);
-              qc.mma(dk, d[i / 4 % 2], i / 4 % 2, i % L::DT);
-              gc.read(cg + (NT - 1) * L::SUB, i / 4 % 2, i % L::DT);
-              qc.read(cq + (NT - 1) * L::SUB, i / 4 % 2, i % L::DT);
-              soft(NT - 1, 2 * i);
-              soft(NT - 1, 2 * i + 1);
-              fence_schedule();
-            }
-            gc.mma(dv, s[NT - 1]);
-            qc.mma(dk, dp[NT - 1]);
-          } else {
-#pragma unroll
-            for (int t = 0; t < NT; t++) {
-              if (t) {
-                qr.read(rq + t * L::SUB);
-                gr.read(rg + t * L::SUB);
-                stats(t);
-              }
-              fence_schedule();
-#pragma unroll
-              for (int ks = 0; ks < L::KS; ks++) scores(t, ks);
-              fence_schedule();
-              gc.read(cg + t * L::SUB);
-              qc.read(cq + t * L::SUB);
-#pragma unroll
-              for (int r = 0; r < 16; r++) soft(t, r);
-              if constexpr (MASKED)
-                mask_block<false>(band, ids, lid + 32 * t, q0 + 32 * t, kj, kid, h, [&](int r, bool drop) {
-                  s[t][r] = drop ? 0.0f : s[t][r];
-                  dp[t][r] = drop ? 0.0f : dp[t][r];
-                });
-              fence_schedule();
-              gc.mma(dv, s[t]);
-              qc.mma(dk, dp[t]);
-            }
+          for (int g = 0; g < 4; g++) {
+            x[g] = *(const f32x4*)(ll + 32 * t + 8 * g + 4 * h);
+            y[g] = *(const f32x4*)(ld + 32 * t + 8 * g + 4 * h);
           }
         };
-        while (qb >= 0 && !it.cut) tile(std::false_type());
-        while (qb >= 0 && !bad) tile(std::true_type());
+        auto scores = [&](int t, int ks) {
+          s[t] = mma_rows<T>(qr.f[ks], kf[ks], s[t]);
+          dp[t] = mma_rows<T>(gr.f[ks], vf[ks], dp[t]);
+        };
+        auto soft = [&](int t, int r) {
+          weight<T, PLAIN>(a, s[t], dp[t], r, slope, cs, x[r >> 2][r & 3], y[r >> 2][r & 3],
+                           q0 + 32 * t + 4 * h + otx_row(r, 0) - kj);
+        };
+        const uint32_t rq = row_q + off, rg = row_g + off, cq = col_q + off, cg = col_g + off;
+        qr.read(rq);
+        gr.read(rg);
+        stats(0);
+        if constexpr (!MASKED && PIPELINED) {
+          // One wave per SIMD: the weights of one block are formed beside the products of the other,
+          // two elements to two products, and fragments are read where others have just been used.
+          fence_schedule();
+#pragma unroll
+          for (int i = 0; i < 8; i++) {
+            scores(0, i % L::KS);
+            qr.read(rq + (NT - 1) * L::SUB, i % L::KS);
+            gr.read(rg + (NT - 1) * L::SUB, i % L::KS);
+            fence_schedule();
+          }
+#pragma unroll
+          for (int i = 0; i < 8; i++) {
+            scores(NT - 1, i % L::KS);
+            gc.read(cg, i / 4 % 2, i % L::DT);
+            qc.read(cq, i / 4 % 2, i % L::DT);
+            soft(0, 2 * i);
+            soft(0, 2 * i + 1);
+            fence_schedule();
+          }
+          stats(NT - 1);
+          typename Cols<T, D>::W p[2] = {gc.weights(s[0], 0), gc.weights(s[0], 1)};
+          typename Cols<T, D>::W d[2] = {qc.weights(dp[0], 0), qc.weights(dp[0], 1)};
+          fence_schedule();
+#pragma unroll
+          for (int i = 0; i < 8; i++) {
+            gc.mma(dv, p[i / 4 % 2], i / 4 % 2, i % L::DT);
+            qc.mma(dk, d[i / 4 % 2], i / 4 % 2, i % L::DT);
+            gc.read(cg + (NT - 1) * L::SUB, i / 4 % 2, i % L::DT);
+            qc.read(cq + (NT - 1) * L::SUB, i / 4 % 2, i % L::DT);
+            soft(NT - 1, 2 * i);
+            soft(NT - 1, 2 * i + 1);
+            fence_schedule();
+          }
+          gc.mma(dv, s[NT - 1]);
+          qc.mma(dk, dp[NT - 1]);
+        } else {
+#pragma unroll
+          for (int t = 0; t < NT; t++) {
+            if (t) {
+              qr.read(rq + t * L::SUB);
+              gr.read(rg + t * L::SUB);
+              stats(t);
+            }
+            fence_schedule();
+#pragma unroll
+            for (int ks = 0; ks < L::KS; ks++) {
+              scores(t, ks);
+              read_step(gc, cg + t * L::SUB, ks);
+              read_step(qc, cq + t * L::SUB, ks);
+            }
+            fence_schedule();
+#pragma unroll
+            for (int r = 0; r < 16; r++) soft(t, r);
+            if (MASKED && rare(cut))
+              mask_block<false>(band, ids, lid + 32 * t, q0 + 32 * t, kj, kid >= 0, kid, h, [&](int r, bool drop) {
+                s[t][r] = drop ? 0.0f : s[t][r];
+                dp[t][r] = drop ? 0.0f : dp[t][r];
+              });
+            fence_schedule();
+            gc.mma(dv, s[t]);
+            qc.mma(dk, dp[t]);
+          }
+        }
+      };
+      while (qb >= 0) {
+        if constexpr (PIPELINED)
+          while (qb >= 0 && !it.cut) tile(std::false_type());
+        while (qb >= 0 && (it.cut || !PIPELINED)) tile(std::true_type());
       }
-      if (rare(bad)) return false;
+      if (rare(met_nonfinite(largest, lbad, seq++))) return false;
       if (kj < S) {
         if constexpr (SPLIT) {
           float* p = a.part + (((long)b * a.H + first) * S + kj) * D;
