@@ -239,6 +239,13 @@ struct Largest {
   }
 };
 
+// x, as a value that is formed here: what rarely run code makes of it does not wait in registers
+// through the loops (it did, and cost them up to 40).
+__device__ __forceinline__ int here(int x) {
+  asm volatile("" : "+v"(x));
+  return x;
+}
+
 // For branches off the common path: registers are kept for the other side.
 __device__ __forceinline__ bool rare(bool x) { return __builtin_expect(x, 0); }
 
@@ -287,24 +294,28 @@ struct TileIter {
     whole = n <= 64 ? whole0 : 0;
     part = n <= 64 ? part0 : 0;
   }
+  __device__ __forceinline__ bool load(const Band& band, const i32x4* table, int nb, int lane) {
+    base += 64;
+    if (base >= n) return false;
+    const int t = base + lane, t0 = t * BT, t1 = t0 + BT - 1;
+    bool a = false, all = false, d = false;
+    if (t < n) {
+      a = OWN_QUERIES ? band.any(o0, o1, t0, t1) : band.any(t0, t1, o0, o1);
+      all = OWN_QUERIES ? band.all(o0, o1, t0, t1) : band.all(t0, t1, o0, o1) && t1 < band.S;
+      if (a && table) {
+        const Docs x = docs_of(table, t0 / kTab, t1 / kTab, nb);
+        a = x.lo <= own.hi && own.lo <= x.hi;
+        d = x.lo != x.hi || own.lo != own.hi || x.pad || own.pad;
+      }
+    }
+    docs = __ballot(d);
+    whole = whole0 = __ballot(a && all && !d);
+    part = part0 = __ballot(a && (!all || d));
+    return true;
+  }
   __device__ __forceinline__ int next(const Band& band, const i32x4* table, int nb, int lane) {
     while (rare((whole | part) == 0)) {
-      base += 64;
-      if (base >= n) return -1;
-      const int t = base + lane, t0 = t * BT, t1 = t0 + BT - 1;
-      bool a = false, all = false, d = false;
-      if (t < n) {
-        a = OWN_QUERIES ? band.any(o0, o1, t0, t1) : band.any(t0, t1, o0, o1);
-        all = OWN_QUERIES ? band.all(o0, o1, t0, t1) : band.all(t0, t1, o0, o1) && t1 < band.S;
-        if (a && table) {
-          const Docs x = docs_of(table, t0 / kTab, t1 / kTab, nb);
-          a = x.lo <= own.hi && own.lo <= x.hi;
-          d = x.lo != x.hi || own.lo != own.hi || x.pad || own.pad;
-        }
-      }
-      docs = __ballot(d);
-      whole = whole0 = __ballot(a && all && !d);
-      part = part0 = __ballot(a && (!all || d));
+      if (!load(band, table, nb, lane)) return -1;
     }
     cut = whole == 0;
     const int i = __builtin_ctzll(cut ? part : whole);
@@ -422,7 +433,7 @@ struct Stage {
 #pragma unroll
       for (int i = 0; i < N; i++) copy_lanes<16>(p + (long)i * RS * stride, off, to + i * kThreads * 16);
     } else {
-      const int r = threadIdx.x / L::NC;
+      const int r = here(threadIdx.x) / L::NC;
 #pragma unroll
       for (int i = 0; i < N; i++)
         copy_lanes<16>(p, off + (min(r + i * RS, last) - r) * stride, to + i * kThreads * 16);
@@ -430,8 +441,9 @@ struct Stage {
   }
   // This thread's share of a tile in LDS.
   __device__ __forceinline__ static void look(const char* lds, Largest<T>& largest) {
+    const char* at = lds + here(threadIdx.x) * 16;
 #pragma unroll
-    for (int i = 0; i < N; i++) largest.take(*(const u32x4*)(lds + (threadIdx.x + i * kThreads) * 16));
+    for (int i = 0; i < N; i++) largest.take(*(const u32x4*)(at + i * kThreads * 16));
     fence_schedule();
   }
 };
@@ -450,24 +462,39 @@ __device__ __forceinline__ void load_own(u32x4 (&f)[D * sizeof(T) / 32], const T
     f[ks] = *(const u32x4*)(base + (long)row * stride + (2 * ks + (lane >> 5)) * (16 / (int)sizeof(T)));
 }
 
-// Writes acc^T (column n = this lane's row) times f into a row of an output tensor.
-template <typename T, int D>
-__device__ __forceinline__ void store_own(T* row, const f32x16 (&acc)[D / 32], float f, int lane) {
+// Writes the 32 rows of a wave: acc^T (column n: row n) times f, to row * stride.  The results pass
+// through this wave's share of LDS, so that 16 bytes a lane go to whole rows: stored as the lanes hold
+// them, 8 bytes to each of 32 rows, they took 3 us of a workgroup's time.
+template <typename T, int D, typename O>
+__device__ __forceinline__ void store_rows(O* out, long stride, int row0, int S, char* lds, const f32x16 (&acc)[D / 32],
+                                           float f) {
+  const int lane = here(threadIdx.x) & 63;
+  constexpr int E = 16 / (int)sizeof(O), C = D / E;  // elements of a chunk, chunks of a row
+  const int n = lane & 31, h = lane >> 5;
 #pragma unroll
   for (int dt = 0; dt < D / 32; dt++)
 #pragma unroll
     for (int g = 0; g < 4; g++) {
-      T* p = row + 32 * dt + 8 * g + 4 * (lane >> 5);
-      if constexpr (sizeof(T) == 2) {
+      const int d = 32 * dt + 8 * g + 4 * h;
+      char* at = lds + n * D * (int)sizeof(O) + (((d / E) ^ (n & (C - 1) & 15)) << 4) + d % E * (int)sizeof(O);
+      if constexpr (sizeof(O) == 2) {
         bf16x4 o;
 #pragma unroll
         for (int i = 0; i < 4; i++) o[i] = (__bf16)(acc[dt][4 * g + i] * f);
-        *(bf16x4*)p = o;
+        *(bf16x4*)at = o;
       } else {
-        *(float4*)p = make_float4(acc[dt][4 * g] * f, acc[dt][4 * g + 1] * f, acc[dt][4 * g + 2] * f,
-                                  acc[dt][4 * g + 3] * f);
+        f32x4 o;
+#pragma unroll
+        for (int i = 0; i < 4; i++) o[i] = acc[dt][4 * g + i] * f;
+        *(f32x4*)at = o;
       }
     }
+#pragma unroll
+  for (int i = 0; i < C / 2; i++) {
+    const int r = (i * 64 + lane) / C, c = (i * 64 + lane) % C;
+    const u32x4 v = *(const u32x4*)(lds + r * D * (int)sizeof(O) + ((c ^ (r & (C - 1) & 15)) << 4));
+    if (row0 + r < S) *(u32x4*)(out + (row0 + r) * stride + c * E) = v;
+  }
 }
 
 // The head that the i-th of n = B * H work items of a row of the grid takes.  Workgroups go round
@@ -542,7 +569,7 @@ template <typename T, int D, int WHAT>
 __device__ __forceinline__ void careful_row(const MaskAttnArgs& a, int b, int head, int hk, int own) {
   constexpr bool KEYS = WHAT == kDKDV || WHAT == kDKDVPart;  // the row is a key
   constexpr int C = D / 64;
-  const int lane = threadIdx.x & 63, S = a.S;
+  const int lane = here(threadIdx.x) & 63, S = a.S;
   const int* doc = a.doc ? a.doc + (long)b * S : nullptr;
   const int prefix = a.prefix ? min(max(a.prefix[b], 0), S) : 0, w = a.window ? a.window : S;
   const T* k = (const T*)a.k + b * a.sk[0] + hk * a.sk[1];
@@ -633,7 +660,8 @@ template <typename T, int D, bool PLAIN>
 __global__ void __launch_bounds__(kThreads, 2) mask_attn_fwd_kernel(const MaskAttnArgs a) {
   using L = Tile<T, D>;
   constexpr int BN = tile_rows<T>(), NT = BN / 32, BM = 128, BYTES = BN * L::RB;
-  __shared__ __align__(1024) char lk_[2][BYTES], lv_[2][BYTES];
+  __shared__ __align__(1024) char tiles[4 * BYTES];
+  char (*lk_)[BYTES] = (char (*)[BYTES])tiles, (*lv_)[BYTES] = lk_ + 2;
   __shared__ __align__(16) int lid_[2][64];
   __shared__ int lbad;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5;
@@ -657,10 +685,6 @@ __global__ void __launch_bounds__(kThreads, 2) mask_attn_fwd_kernel(const MaskAt
     gv.init((const T*)a.v + b * a.sv[0] + hk * a.sv[1], a.sv[2]);
 
     const Docs own = docs_of(table, q0 / kTab, q1 / kTab, nb);
-    u32x4 qf[L::KS];
-    load_own<T, D>(qf, (const T*)a.q + b * a.sq[0] + hq * a.sq[1], a.sq[2], min(qi, S - 1), lane);
-    const int qid = doc ? doc[min(qi, S - 1)] : 0;
-
     // False, with nothing written, where a tile holds a non-finite value that some row does not see.
     auto item = [&]() {
       TileIter<BN, true> it;
@@ -674,6 +698,9 @@ __global__ void __launch_bounds__(kThreads, 2) mask_attn_fwd_kernel(const MaskAt
       };
       arrived();  // the last item's tiles have been read, and no copy is on its way
       if (kb >= 0) stage();
+      u32x4 qf[L::KS];
+      load_own<T, D>(qf, (const T*)a.q + b * a.sq[0] + hq * a.sq[1], a.sq[2], min(qi, S - 1), lane);
+      const int qid = doc ? doc[min(qi, S - 1)] : 0;
       f32x16 acc[L::DT] = {};
       float m = -INFINITY, l = 0.0f;
 
@@ -780,14 +807,12 @@ __global__ void __launch_bounds__(kThreads, 2) mask_attn_fwd_kernel(const MaskAt
       while (kb >= 0) tile();
       if (rare(met_nonfinite(largest, lbad, seq++))) return false;
       l = sum_halves(l);
-      if (qi < S) {
-        store_own<T, D>((T*)a.out + b * a.so[0] + hq * a.so[1] + qi * a.so[2], acc, l == 0.0f ? 0.0f : 1.0f / l, lane);
-        if (h == 0) a.lse[((long)b * a.H + hq) * S + qi] = l == 0.0f ? 0.0f : m + __builtin_log2f(l);
-      }
+      if (qi < S && h == 0) a.lse[((long)b * a.H + hq) * S + qi] = l == 0.0f ? 0.0f : m + __builtin_log2f(l);
+      store_rows<T, D>((T*)a.out + b * a.so[0] + hq * a.so[1], a.so[2], qw0, S, tiles + wave * 32 * L::RB, acc,
+                       l == 0.0f ? 0.0f : 1.0f / l);
       return true;
     };
     if (rare(!item())) {
-      arrived();
       for (int i = qw0; i <= qw1; i++) careful_row<T, D, kForward>(a, b, hq, hk, i);
     }
   }
@@ -798,7 +823,8 @@ template <typename T, int D, bool PLAIN>
 __global__ void __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) mask_attn_dq_kernel(const MaskAttnArgs a) {
   using L = Tile<T, D>;
   constexpr int BN = tile_rows<T>(), NT = BN / 32, BM = 128, BYTES = BN * L::RB;
-  __shared__ __align__(1024) char lk_[2][BYTES], lv_[2][BYTES];
+  __shared__ __align__(1024) char tiles[4 * BYTES];
+  char (*lk_)[BYTES] = (char (*)[BYTES])tiles, (*lv_)[BYTES] = lk_ + 2;
   __shared__ __align__(16) int lid_[2][64];
   __shared__ int lbad;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5;
@@ -823,25 +849,6 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) mask_attn_dq
     gv.init((const T*)a.v + b * a.sv[0] + hk * a.sv[1], a.sv[2]);
 
     const Docs own = docs_of(table, q0 / kTab, q1 / kTab, nb);
-    u32x4 qf[L::KS], gf[L::KS];
-    load_own<T, D>(qf, (const T*)a.q + b * a.sq[0] + hq * a.sq[1], a.sq[2], qr, lane);
-    load_own<T, D>(gf, (const T*)a.dout + b * a.sdo[0] + hq * a.sdo[1], a.sdo[2], qr, lane);
-    float dsum = 0.0f;
-    {
-      const T* op = (const T*)a.o + b * a.so[0] + hq * a.so[1] + qr * a.so[2];
-#pragma unroll
-      for (int ks = 0; ks < L::KS; ks++) {
-        const u32x4 of = *(const u32x4*)(op + (2 * ks + h) * (16 / (int)sizeof(T)));
-#pragma unroll
-        for (int e = 0; e < Elem<T>::VEC; e++)
-          dsum = __builtin_fmaf(element<T>(gf[ks], e), element<T>(of, e), dsum);
-      }
-      dsum = sum_halves(dsum);
-    }
-    const long row = ((long)b * a.H + hq) * S + qr;
-    if (qi < S && h == 0) a.dsum[row] = dsum;
-    const float lse = a.lse[row];
-    const int qid = doc ? doc[min(qi, S - 1)] : 0;
     auto item = [&]() {
       TileIter<BN, true> it;
       it.init(q0, q1, own, nk);
@@ -852,8 +859,27 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) mask_attn_dq
         gv.copy(lv_[buf], kb * BN, S);
         if (doc && wave == 0) copy_lanes<4>(doc, min(kb * BN + lane, S - 1) * 4, lds_address(lid_[buf]));
       };
-      arrived();
+      __syncthreads();  // the last item is done with LDS
       if (kb >= 0) stage();
+      u32x4 qf[L::KS], gf[L::KS];
+      load_own<T, D>(qf, (const T*)a.q + b * a.sq[0] + hq * a.sq[1], a.sq[2], qr, lane);
+      load_own<T, D>(gf, (const T*)a.dout + b * a.sdo[0] + hq * a.sdo[1], a.sdo[2], qr, lane);
+      float dsum = 0.0f;
+      {
+        const T* op = (const T*)a.o + b * a.so[0] + hq * a.so[1] + qr * a.so[2];
+#pragma unroll
+        for (int ks = 0; ks < L::KS; ks++) {
+          const u32x4 of = *(const u32x4*)(op + (2 * ks + h) * (16 / (int)sizeof(T)));
+#pragma unroll
+          for (int e = 0; e < Elem<T>::VEC; e++)
+            dsum = __builtin_fmaf(element<T>(gf[ks], e), element<T>(of, e), dsum);
+        }
+        dsum = sum_halves(dsum);
+      }
+      const long row = ((long)b * a.H + hq) * S + qr;
+      if (qi < S && h == 0) a.dsum[row] = dsum;
+      const float lse = a.lse[row];
+      const int qid = doc ? doc[min(qi, S - 1)] : 0;
       f32x16 acc[L::DT] = {};
 
       auto tile = [&]() {
@@ -898,11 +924,10 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) mask_attn_dq
       };
       while (kb >= 0) tile();
       if (rare(met_nonfinite(largest, lbad, seq++))) return false;
-      if (qi < S) store_own<T, D>((T*)a.dq + b * a.sdq[0] + hq * a.sdq[1] + qi * a.sdq[2], acc, a.sigma, lane);
+      store_rows<T, D>((T*)a.dq + b * a.sdq[0] + hq * a.sdq[1], a.sdq[2], qw0, S, tiles + wave * 32 * L::RB, acc, a.sigma);
       return true;
     };
     if (rare(!item())) {
-      arrived();
       for (int i = qw0; i <= qw1; i++) careful_row<T, D, kDQ>(a, b, hq, hk, i);
     }
   }
@@ -916,7 +941,8 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) * D == 128 ? 2 : 1) mask_a
   using L = Tile<T, D>;
   constexpr int BN = tile_rows<T>(), NT = BN / 32, BM = 128, BYTES = BN * L::RB;  // BM keys owned, BN queries a tile
   constexpr bool PIPELINED = NT == 2 && L::KS == 8 && L::DT == 4;
-  __shared__ __align__(1024) char lq_[2][BYTES], lg_[2][BYTES];
+  __shared__ __align__(1024) char tiles[4 * BYTES];
+  char (*lq_)[BYTES] = (char (*)[BYTES])tiles, (*lg_)[BYTES] = lq_ + 2;
   __shared__ __align__(16) float ll_[2][64], ld_[2][64];
   __shared__ __align__(16) int lid_[2][64];
   __shared__ int lbad;
@@ -931,20 +957,15 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) * D == 128 ? 2 : 1) mask_a
   int seq = 0;
 
   for (long w = blockIdx.x; w < total; w += gridDim.x) {
-    const int bh = spread((int)(w % (a.B * heads)), a.B * heads), b = bh / heads;
-    const int hk = SPLIT ? bh % heads / group : bh % heads;
-    const int k0 = (int)(w / (a.B * heads)) * BM, k1 = min(k0 + BM, S) - 1;  // the first keys have the most queries
+    // the first keys have the most queries, so they come first
+    const int bh = (int)(w % ((long)a.B * heads)), b = bh / heads, head = bh % heads, hk = SPLIT ? head / group : head;
+    const int k0 = (int)(w / ((long)a.B * heads)) * BM, k1 = min(k0 + BM, S) - 1;
     const int kw0 = k0 + 32 * wave, kw1 = min(kw0 + 31, S - 1), kj = kw0 + (lane & 31), kr = min(kj, S - 1);
     const int* doc = a.doc ? a.doc + (long)b * S : nullptr;
     const i32x4* table = a.doc ? (const i32x4*)a.table + (long)b * nb : nullptr;
     const Band band = {S, a.window, a.prefix ? min(max(a.prefix[b], 0), S) : 0};
     const Docs own = docs_of(table, k0 / kTab, k1 / kTab, nb);
-
-    u32x4 kf[L::KS], vf[L::KS];
-    load_own<T, D>(kf, (const T*)a.k + b * a.sk[0] + hk * a.sk[1], a.sk[2], kr, lane);
-    load_own<T, D>(vf, (const T*)a.v + b * a.sv[0] + hk * a.sv[1], a.sv[2], kr, lane);
-    const int kid = doc ? doc[kr] : 0;
-    const int first = SPLIT ? bh % heads : hk * group, last = SPLIT ? first + 1 : first + group;
+    const int first = SPLIT ? head : hk * group, last = SPLIT ? first + 1 : first + group;
 
     auto item = [&]() {
       f32x16 dk[L::DT] = {}, dv[L::DT] = {};
@@ -967,9 +988,13 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) * D == 128 ? 2 : 1) mask_a
         if (wave == 1) copy_lanes<4>(a.dsum + row0, i, lds_address(ld_[buf]));
         if (doc && wave == 2) copy_lanes<4>(doc, i, lds_address(lid_[buf]));
       };
-      arrived();
+      __syncthreads();  // the last item is done with LDS
       take_head();
       if (qb >= 0) stage();
+      u32x4 kf[L::KS], vf[L::KS];
+      load_own<T, D>(kf, (const T*)a.k + b * a.sk[0] + hk * a.sk[1], a.sk[2], kr, lane);
+      load_own<T, D>(vf, (const T*)a.v + b * a.sv[0] + hk * a.sv[1], a.sv[2], kr, lane);
+      const int kid = doc ? doc[kr] : 0;
 
       auto tile = [&](auto masks) {
       constexpr bool MASKED = decltype(masks)::value;
@@ -1088,20 +1113,19 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) * D == 128 ? 2 : 1) mask_a
         while (qb >= 0 && (it.cut || !PIPELINED)) tile(std::true_type());
       }
       if (rare(met_nonfinite(largest, lbad, seq++))) return false;
-      if (kj < S) {
-        if constexpr (SPLIT) {
-          float* p = a.part + (((long)b * a.H + first) * S + kj) * D;
-          store_own<float, D>(p, dk, a.sigma, lane);
-          store_own<float, D>(p + (long)a.B * a.H * S * D, dv, 1.0f, lane);
-        } else {
-          store_own<T, D>((T*)a.dk + b * a.sdk[0] + hk * a.sdk[1] + kj * a.sdk[2], dk, a.sigma, lane);
-          store_own<T, D>((T*)a.dv + b * a.sdv[0] + hk * a.sdv[1] + kj * a.sdv[2], dv, 1.0f, lane);
-        }
+      if constexpr (SPLIT) {
+        float* p = a.part + ((long)b * a.H + first) * S * D;
+        char* lds = tiles + wave * 32 * 4 * D;
+        store_rows<T, D>(p, D, kw0, S, lds, dk, a.sigma);
+        store_rows<T, D>(p + (long)a.B * a.H * S * D, D, kw0, S, lds, dv, 1.0f);
+      } else {
+        char* lds = tiles + wave * 32 * L::RB;
+        store_rows<T, D>((T*)a.dk + b * a.sdk[0] + hk * a.sdk[1], a.sdk[2], kw0, S, lds, dk, a.sigma);
+        store_rows<T, D>((T*)a.dv + b * a.sdv[0] + hk * a.sdv[1], a.sdv[2], kw0, S, lds, dv, 1.0f);
       }
       return true;
     };
     if (rare(!item())) {
-      arrived();
       for (int j = kw0; j <= kw1; j++) careful_row<T, D, SPLIT ? kDKDVPart : kDKDV>(a, b, first, hk, j);
     }
   }
