@@ -52,9 +52,9 @@ hipError_t launch_mask_table(const int* doc, void* table, int B, int S, hipStrea
 hipError_t launch_mask_attn(int dtype, int D, bool backward, const MaskAttnArgs& a, hipStream_t st);
 hipError_t launch_rotary(int dtype, const RotaryArgs& a, bool half, bool wide, hipStream_t st);
 int layer_norm_parts(long rows, int D);
-hipError_t launch_layer_norm_fwd(int dtype, bool wide, const void* x, const void* w, const void* b, void* y,
+hipError_t launch_layer_norm_fwd(int dtype, const void* x, const void* w, const void* b, void* y,
                                  float* mean, float* rstd, long rows, int D, float eps, hipStream_t st);
-hipError_t launch_layer_norm_bwd(int dtype, bool wide, const void* x, const void* w, const float* mean,
+hipError_t launch_layer_norm_bwd(int dtype, const void* x, const void* w, const float* mean,
                                  const float* rstd, const void* dy, void* dx, void* dw, void* db, int wdtype,
                                  float* part, long rows, int D, hipStream_t st);
 }  // namespace otx
@@ -928,8 +928,7 @@ int otx_layer_norm_fwd(const void* x, const void* w, const void* b, void* y, flo
   int rc = check_layer_norm(rows, D, dtype);
   if (rc) return rc;
   if (!x || !w || !y || !mean || !rstd) return fail(OTX_EINVAL, "null pointer argument");
-  const bool wide = D % (dtype == OTX_DTYPE_BF16 ? 8 : 4) == 0 && aligned16(x) && aligned16(w) && aligned16(b) && aligned16(y);
-  hipError_t e = otx::launch_layer_norm_fwd(dtype, wide, x, w, b, y, mean, rstd, rows, D, eps, (hipStream_t)stream);
+  hipError_t e = otx::launch_layer_norm_fwd(dtype, x, w, b, y, mean, rstd, rows, D, eps, (hipStream_t)stream);
   return e == hipSuccess ? OTX_OK : fail(OTX_EHIP, "layer norm launch failed: %s", hipGetErrorString(e));
 }
 
@@ -949,8 +948,7 @@ int otx_layer_norm_bwd(const void* x, const void* w, const float* mean, const fl
   const size_t need = otx_layer_norm_bwd_workspace_bytes(rows, D);
   if (workspace_bytes < need)
     return fail(OTX_EINVAL, "workspace too small: %zu bytes given, %zu needed", workspace_bytes, need);
-  const bool wide = D % (dtype == OTX_DTYPE_BF16 ? 8 : 4) == 0 && aligned16(x) && aligned16(w) && aligned16(dy) && aligned16(dx);
-  hipError_t e = otx::launch_layer_norm_bwd(dtype, wide, x, w, mean, rstd, dy, dx, dw, db, wdtype, (float*)workspace,
+  hipError_t e = otx::launch_layer_norm_bwd(dtype, x, w, mean, rstd, dy, dx, dw, db, wdtype, (float*)workspace,
                                             rows, D, (hipStream_t)stream);
   return e == hipSuccess ? OTX_OK : fail(OTX_EHIP, "layer norm backward launch failed: %s", hipGetErrorString(e));
 }
