@@ -50,7 +50,7 @@ hipError_t launch_swap_heads(int dtype, const void* in, void* out, int B, int X,
 bool mask_attn_splits(int B, int H, int Hkv, int S);
 hipError_t launch_mask_table(const int* doc, void* table, int B, int S, hipStream_t st);
 hipError_t launch_mask_attn(int dtype, int D, bool backward, const MaskAttnArgs& a, hipStream_t st);
-hipError_t launch_rotary(int dtype, const RotaryArgs& a, bool half, bool wide, hipStream_t st);
+hipError_t launch_rotary(int dtype, const RotaryArgs& a, bool half, hipStream_t st);
 int layer_norm_parts(long rows, int D);
 hipError_t launch_layer_norm_fwd(int dtype, const void* x, const void* w, const void* b, void* y,
                                  float* mean, float* rstd, long rows, int D, float eps, hipStream_t st);
@@ -900,17 +900,14 @@ int otx_rotary(const void* x, const float* cosv, const float* sinv, const int32_
   if (x == y) return fail(OTX_EINVAL, "rotary: the output must not alias the input");
   if (D > (1 << 20) || H > 65535 || (long long)B * T * (D / 2 + 1) >= 0x80000000LL)
     return fail(OTX_EINVAL, "rotary: tensor too large");
-  const int vec = dtype == OTX_DTYPE_BF16 ? 8 : 4;
   otx::RotaryArgs a = {};
-  bool wide = D % vec == 0 && R % (2 * vec) == 0 && aligned16(x) && aligned16(y) && aligned16(cosv) && aligned16(sinv);
   for (int i = 0; i < 3; i++) {
     a.sx[i] = strides[i], a.sy[i] = strides[3 + i];
     if (a.sx[i] < 0 || a.sy[i] < 0) return fail(OTX_EINVAL, "rotary: negative stride");
-    wide = wide && a.sx[i] % vec == 0 && a.sy[i] % vec == 0;
   }
   a.x = x, a.y = y, a.cosv = cosv, a.sinv = sinv, a.positions = positions;
   a.B = B, a.T = T, a.H = H, a.D = D, a.R = R, a.P = P, a.sign = backward ? -1.0f : 1.0f;
-  hipError_t e = otx::launch_rotary(dtype, a, layout == 1, wide, (hipStream_t)stream);
+  hipError_t e = otx::launch_rotary(dtype, a, layout == 1, (hipStream_t)stream);
   return e == hipSuccess ? OTX_OK : fail(OTX_EHIP, "rotary launch failed: %s", hipGetErrorString(e));
 }
 

@@ -4,7 +4,7 @@
 // are copied.  The gradient is the transpose, the same kernel with -s.
 //
 // Bound by memory: x is read once and written once, in the other order of heads and rows.  A thread
-// takes one unit of V pairs (two accesses of 16 bytes) of a row, and the same unit of several heads,
+// takes one unit of V pairs (two accesses of up to 16 bytes, at any address) of a row, and the same unit of several heads,
 // so that the position, c and s are read once for all of them.
 #include "otx_args.h"
 #include "otx_common.h"
@@ -13,6 +13,11 @@ namespace otx {
 
 namespace {
 
+// N bytes, to be read and written at any address.
+template <int N> struct Bytes { typedef uint32_t __attribute__((ext_vector_type(N / 4))) V; typedef V At __attribute__((aligned(2))); };
+template <> struct Bytes<4> { typedef uint32_t V; typedef V At __attribute__((aligned(2))); };
+template <> struct Bytes<2> { typedef uint16_t V, At; };
+
 template <typename T, int V>
 struct Vec {
   T e[V];
@@ -20,37 +25,26 @@ struct Vec {
 
 template <typename T, int V>
 __device__ __forceinline__ void load(const T* p, float (&f)[V]) {
-  if constexpr (V == 1) {
-    f[0] = Elem<T>::ld(p);
-  } else {
-    const uint4 w = *(const uint4*)p;
+  typedef Bytes<V * sizeof(T)> Raw;
+  const auto v = __builtin_bit_cast(Vec<T, V>, (typename Raw::V)*(const typename Raw::At*)p);
 #pragma unroll
-    for (int i = 0; i < V; i++) f[i] = Elem<T>::get(w, i);
-  }
+  for (int i = 0; i < V; i++) f[i] = Elem<T>::ld(v.e + i);
 }
 
 template <typename T, int V>
 __device__ __forceinline__ void store(T* p, const float (&f)[V]) {
+  typedef Bytes<V * sizeof(T)> Raw;
   Vec<T, V> v;
 #pragma unroll
   for (int i = 0; i < V; i++) v.e[i] = Elem<T>::put(f[i]);
-  if constexpr (V == 1)
-    *p = v.e[0];
-  else
-    *(uint4*)p = __builtin_bit_cast(uint4, v);
+  *(typename Raw::At*)p = __builtin_bit_cast(typename Raw::V, v);
 }
 
 template <int V>
 __device__ __forceinline__ void load_table(const float* p, float (&f)[V]) {
-  if constexpr (V == 1) {
-    f[0] = *p;
-  } else {
+  constexpr int W = V < 4 ? V : 4;
 #pragma unroll
-    for (int i = 0; i < V; i += 4) {
-      const float4 w = *(const float4*)(p + i);
-      f[i] = w.x, f[i + 1] = w.y, f[i + 2] = w.z, f[i + 3] = w.w;
-    }
-  }
+  for (int i = 0; i < V; i += W) load<float, W>(p + i, *(float (*)[W])(f + i));
 }
 
 template <typename T, int V, bool HALF>
@@ -63,14 +57,14 @@ __global__ void __launch_bounds__(256) rotary_kernel(const RotaryArgs a, int hea
     T* y = (T*)a.y + b * a.sy[0] + t * a.sy[1];
     if (u >= turned) {  // columns that are not turned
       const int first = a.R + (int)(u - turned) * 2 * V;
+      const int second = first + V < a.D ? first + V : first;
+#pragma unroll 4
       for (int h = h0; h < h1; h++) {
-        float f[V];
+        float f[V], g[V];
         load<T, V>(x + h * a.sx[2] + first, f);
+        load<T, V>(x + h * a.sx[2] + second, g);
         store<T, V>(y + h * a.sy[2] + first, f);
-        if (first + V < a.D) {
-          load<T, V>(x + h * a.sx[2] + first + V, f);
-          store<T, V>(y + h * a.sy[2] + first + V, f);
-        }
+        store<T, V>(y + h * a.sy[2] + second, g);
       }
       continue;
     }
@@ -133,10 +127,16 @@ hipError_t rotary_of(const RotaryArgs& a, bool half, hipStream_t st) {
 
 }  // namespace
 
-// wide: every access can be of 16 bytes (V elements divide D, 2 V divide R, aligned rows).
-hipError_t launch_rotary(int dtype, const RotaryArgs& a, bool half, bool wide, hipStream_t st) {
-  if (dtype == 1) return wide ? rotary_of<uint16_t, 8>(a, half, st) : rotary_of<uint16_t, 1>(a, half, st);
-  return wide ? rotary_of<float, 4>(a, half, st) : rotary_of<float, 1>(a, half, st);
+// Wide accesses where the turned and the copied columns divide into them.  8192 rows of 16 heads, 24 of
+// 96 bf16 columns turned: 15 us by 4, 22 by 1 (by 2, as 20 of 80 allows, 20 and 22: not worth its code);
+// 128 of 128 by 8: 13 us, its traffic at 5.2 TB/s.
+hipError_t launch_rotary(int dtype, const RotaryArgs& a, bool half, hipStream_t st) {
+  const int odd = a.R / 2 | (a.D - a.R);  // V divides both
+  if (dtype == 1) {
+    if (odd % 8 == 0) return rotary_of<uint16_t, 8>(a, half, st);
+    return odd % 4 == 0 ? rotary_of<uint16_t, 4>(a, half, st) : rotary_of<uint16_t, 1>(a, half, st);
+  }
+  return odd % 4 == 0 ? rotary_of<float, 4>(a, half, st) : rotary_of<float, 1>(a, half, st);
 }
 
 }  // namespace otx
