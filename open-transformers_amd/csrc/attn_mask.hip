@@ -278,15 +278,15 @@ __device__ __forceinline__ Docs docs_of(const i32x4* table, int first, int last,
 // The tiles of BT tokens that a range of `own` tokens meets, 64 at a time (a lane tests one): of these
 // first the ones that all of the range sees whole, then those that the mask cuts, so that the loop over
 // whole tiles holds no mask.
-template <int BT, bool OWN_QUERIES>
+template <int BT, bool OWN_QUERIES, bool TEAM>  // TEAM: every fourth tile, dealt to the waves in turn
 struct TileIter {
   uint64_t whole, part, docs;  // docs: tiles whose pairs need not be of one document
   uint64_t whole0, part0;
-  int base, n, o0, o1;
+  int base, n, o0, o1, seen;
   bool cut, mixed;  // of the tile that next() returned
   Docs own;
   __device__ __forceinline__ void init(int own0, int own1, const Docs& d, int ntiles) {
-    o0 = own0, o1 = own1, own = d, n = ntiles, whole = part = 0, base = -64, cut = mixed = false;
+    o0 = own0, o1 = own1, own = d, n = ntiles, whole = part = 0, base = -64, cut = mixed = false, seen = 0;
   }
   // Starts over for the same range.
   __device__ __forceinline__ void again() {
@@ -311,6 +311,13 @@ struct TileIter {
     docs = __ballot(d);
     whole = whole0 = __ballot(a && all && !d);
     part = part0 = __ballot(a && (!all || d));
+    if constexpr (TEAM) {
+      const uint64_t below = (1ull << lane) - 1;
+      const int rank = (whole >> lane) & 1 ? __popcll(whole & below) : __popcll(whole) + __popcll(part & below);
+      const uint64_t mine = __ballot(((rank + seen) & 3) == (int)(threadIdx.x >> 6));
+      seen += __popcll(whole | part);
+      whole &= mine, part &= mine;
+    }
     return true;
   }
   __device__ __forceinline__ int next(const Band& band, const i32x4* table, int nb, int lane) {
@@ -414,36 +421,41 @@ __device__ __forceinline__ uint32_t lds_address(const void* p) {
 // BT rows of a tensor, copied straight into LDS (16 bytes a lane, no registers); rows past the end
 // repeat the last one.  A wave's copy fills consecutive LDS, so the swizzle is applied to the chunk
 // that a lane fetches.
-template <typename T, int D, int BT>
+template <typename T, int D, int BT, bool TEAM>  // TEAM: the lanes of one wave; otherwise the whole workgroup
 struct Stage {
   using L = Tile<T, D>;
-  static constexpr int N = BT * L::NC / kThreads, RS = kThreads / L::NC;  // steps, rows a step
-  static_assert(BT * L::NC % kThreads == 0 && RS % (L::SW + 1) == 0, "a step keeps the swizzle");
+  static constexpr int NTH = TEAM ? 64 : kThreads;
+  static constexpr int N = BT * L::NC / NTH, RS = NTH / L::NC;  // steps, rows a step
+  static_assert(BT * L::NC % NTH == 0, "whole steps");
   const char* base;
-  int stride, off;  // bytes
+  int stride, off, row, col;  // bytes, but for row
   __device__ __forceinline__ void init(const T* p, long s) {
-    const int r = threadIdx.x / L::NC, c = (threadIdx.x % L::NC) ^ L::swizzle(r);
-    base = (const char*)p, stride = (int)s * (int)sizeof(T), off = r * stride + c * 16;
+    const int r = threadIdx.x % NTH / L::NC;
+    row = r, col = ((threadIdx.x % L::NC) ^ L::swizzle(r)) * 16;
+    base = (const char*)p, stride = (int)s * (int)sizeof(T), off = r * stride + col;
   }
+  // From the chunk that this lane fetches in the first step to that of step i: the swizzle's bits are
+  // exclusive-ors of the row's, so that of row r + i RS is that of r with that of i RS.
+  __device__ __forceinline__ int turn(int i) const { return (col ^ (L::swizzle(i * RS) << 4)) - col; }
   __device__ __forceinline__ void copy(char* lds, int row0, int S) const {
     const char* p = base + (long)row0 * stride;
-    const uint32_t to = lds_address(lds) + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) * 1024;
+    const uint32_t to = lds_address(lds) + (TEAM ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) * 1024);
     const int last = S - 1 - row0;
     if (!rare(last < BT - 1)) {
 #pragma unroll
-      for (int i = 0; i < N; i++) copy_lanes<16>(p + (long)i * RS * stride, off, to + i * kThreads * 16);
+      for (int i = 0; i < N; i++) copy_lanes<16>(p + (long)i * RS * stride, off + turn(i), to + i * NTH * 16);
     } else {
-      const int r = here(threadIdx.x) / L::NC;
+      const int r = here(row);
 #pragma unroll
       for (int i = 0; i < N; i++)
-        copy_lanes<16>(p, off + (min(r + i * RS, last) - r) * stride, to + i * kThreads * 16);
+        copy_lanes<16>(p, off + (min(r + i * RS, last) - r) * stride + turn(i), to + i * NTH * 16);
     }
   }
   // This thread's share of a tile in LDS.
   __device__ __forceinline__ static void look(const char* lds, Largest<T>& largest) {
-    const char* at = lds + here(threadIdx.x) * 16;
+    const char* at = lds + here(threadIdx.x) % NTH * 16;
 #pragma unroll
-    for (int i = 0; i < N; i++) largest.take(*(const u32x4*)(at + i * kThreads * 16));
+    for (int i = 0; i < N; i++) largest.take(*(const u32x4*)(at + i * NTH * 16));
     fence_schedule();
   }
 };
@@ -453,6 +465,11 @@ __device__ __forceinline__ void arrived() {
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   __builtin_amdgcn_s_waitcnt(0x0f70);  // the same for the compiler, which has its own loads counted as done
   __syncthreads();
+}
+// The same for a wave with tiles of its own, which has also read what the next copies overwrite.
+__device__ __forceinline__ void arrived_here() {
+  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+  __builtin_amdgcn_s_waitcnt(0x0070);
 }
 
 template <typename T, int D>
@@ -494,6 +511,46 @@ __device__ __forceinline__ void store_rows(O* out, long stride, int row0, int S,
     const int r = (i * 64 + lane) / C, c = (i * 64 + lane) % C;
     const u32x4 v = *(const u32x4*)(lds + r * D * (int)sizeof(O) + ((c ^ (r & (C - 1) & 15)) << 4));
     if (row0 + r < S) *(u32x4*)(out + (row0 + r) * stride + c * E) = v;
+  }
+}
+
+// The same for a team, whose four waves hold summands of the same 32 rows: added in the waves' order.
+template <typename T, int D, typename O>
+__device__ __forceinline__ void join_rows(O* out, long stride, int row0, int S, char* lds, const f32x16 (&acc)[D / 32],
+                                          float f) {
+  constexpr int C = D / 4, PART = 32 * D * 4;  // chunks of four columns in a row, bytes of a wave's summand
+  const int tid = here(threadIdx.x), lane = tid & 63, n = lane & 31, h = lane >> 5;
+  char* mine = lds + (tid >> 6) * PART;
+  __syncthreads();  // LDS is read no more
+#pragma unroll
+  for (int dt = 0; dt < D / 32; dt++)
+#pragma unroll
+    for (int g = 0; g < 4; g++) {
+      const int c = (32 * dt + 8 * g + 4 * h) / 4;
+      f32x4 o;
+#pragma unroll
+      for (int i = 0; i < 4; i++) o[i] = acc[dt][4 * g + i] * f;
+      *(f32x4*)(mine + n * D * 4 + ((c ^ (n & 15)) << 4)) = o;
+    }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < 32 * C / kThreads; i++) {
+    const int r = (i * kThreads + tid) / C, c = (i * kThreads + tid) % C;
+    const char* at = lds + r * D * 4 + ((c ^ (r & 15)) << 4);
+    f32x4 o = *(const f32x4*)at;
+#pragma unroll
+    for (int w = 1; w < 4; w++) o += *(const f32x4*)(at + w * PART);
+    if (row0 + r < S) {
+      O* to = out + (row0 + r) * stride + c * 4;
+      if constexpr (sizeof(O) == 2) {
+        bf16x4 v;
+#pragma unroll
+        for (int e = 0; e < 4; e++) v[e] = (__bf16)o[e];
+        *(bf16x4*)to = v;
+      } else {
+        *(f32x4*)to = o;
+      }
+    }
   }
 }
 
@@ -656,15 +713,18 @@ __device__ __forceinline__ bool met_nonfinite(const Largest<T>& largest, int& lb
 
 // ---- forward -------------------------------------------------------------------------------------
 // Tiles are copied one ahead into the other of two buffers, with one barrier a tile.
-template <typename T, int D, bool PLAIN>
-__global__ void __launch_bounds__(kThreads, 2) mask_attn_fwd_kernel(const MaskAttnArgs a) {
+template <typename T, int D, bool PLAIN, bool TEAM>
+__global__ void __launch_bounds__(kThreads, TEAM || sizeof(T) * D == 512 ? 1 : 2) mask_attn_fwd_kernel(const MaskAttnArgs a) {
   using L = Tile<T, D>;
-  constexpr int BN = tile_rows<T>(), NT = BN / 32, BM = 128, BYTES = BN * L::RB;
-  __shared__ __align__(1024) char tiles[4 * BYTES];
-  char (*lk_)[BYTES] = (char (*)[BYTES])tiles, (*lv_)[BYTES] = lk_ + 2;
-  __shared__ __align__(16) int lid_[2][64];
+  constexpr int BN = TEAM ? 32 : tile_rows<T>(), NT = BN / 32, BM = TEAM ? 32 : 128, BYTES = BN * L::RB;
+  constexpr int NB = TEAM && L::RB == 512 ? 1 : 2, SETS = TEAM ? 4 : 1;  // buffers, and sets of them
+  __shared__ __align__(1024) char tiles[SETS * 2 * NB * BYTES];
+  __shared__ __align__(16) int lids[SETS][2][64];
   __shared__ int lbad;
+  __shared__ float lml[SETS][64];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5;
+  const int set = TEAM ? wave : 0;
+  char (*lk_)[BYTES] = (char (*)[BYTES])tiles + set * 2 * NB, (*lv_)[BYTES] = lk_ + NB;
   const int S = a.S, nq = (S + BM - 1) / BM, nk = (S + BN - 1) / BN, nb = (S + kTab - 1) / kTab;
   const long total = (long)a.B * a.H * nq;
   const float cs = a.sigma * kLog2e;
@@ -675,26 +735,26 @@ __global__ void __launch_bounds__(kThreads, 2) mask_attn_fwd_kernel(const MaskAt
   for (long w = blockIdx.x; w < total; w += gridDim.x) {
     const int bh = spread((int)(w % (a.B * a.H)), a.B * a.H), b = bh / a.H, hq = bh % a.H, hk = hq / (a.H / a.Hkv);
     const int q0 = (nq - 1 - (int)(w / (a.B * a.H))) * BM, q1 = min(q0 + BM, S) - 1;
-    const int qw0 = q0 + 32 * wave, qw1 = min(qw0 + 31, S - 1), qi = qw0 + (lane & 31);
+    const int qw0 = q0 + (TEAM ? 0 : 32 * wave), qw1 = min(qw0 + 31, S - 1), qi = qw0 + (lane & 31);
     const int* doc = a.doc ? a.doc + (long)b * S : nullptr;
     const i32x4* table = a.doc ? (const i32x4*)a.table + (long)b * nb : nullptr;
     const Band band = {S, a.window, a.prefix ? min(max(a.prefix[b], 0), S) : 0};
     const float slope = !PLAIN && a.slopes ? a.slopes[hq] * kLog2e : 0.0f;
-    Stage<T, D, BN> gk, gv;
+    Stage<T, D, BN, TEAM> gk, gv;
     gk.init((const T*)a.k + b * a.sk[0] + hk * a.sk[1], a.sk[2]);
     gv.init((const T*)a.v + b * a.sv[0] + hk * a.sv[1], a.sv[2]);
 
     const Docs own = docs_of(table, q0 / kTab, q1 / kTab, nb);
     // False, with nothing written, where a tile holds a non-finite value that some row does not see.
     auto item = [&]() {
-      TileIter<BN, true> it;
+      TileIter<BN, true, TEAM> it;
       it.init(q0, q1, own, nk);
       int kb = it.next(band, table, nb, lane), buf = 0;
       Largest<T> largest;  // of cut tiles: with an infinity among them, what is formed here is not used
       auto stage = [&]() {
         gk.copy(lk_[buf], kb * BN, S);
         gv.copy(lv_[buf], kb * BN, S);
-        if (doc && wave == 0) copy_lanes<4>(doc, min(kb * BN + lane, S - 1) * 4, lds_address(lid_[buf]));
+        if (doc && (TEAM || wave == 0)) copy_lanes<4>(doc, min(kb * BN + lane, S - 1) * 4, lds_address(lids[set][buf]));
       };
       arrived();  // the last item's tiles have been read, and no copy is on its way
       if (kb >= 0) stage();
@@ -704,16 +764,19 @@ __global__ void __launch_bounds__(kThreads, 2) mask_attn_fwd_kernel(const MaskAt
       f32x16 acc[L::DT] = {};
       float m = -INFINITY, l = 0.0f;
 
+      auto advance = [&]() {
+        kb = it.next(band, table, nb, lane);
+        buf ^= NB - 1;
+        if (kb >= 0) stage();
+      };
       auto tile = [&]() {
         const char* lv = lv_[buf];
         const uint32_t ak = row_k + buf * BYTES, av = col_v + buf * BYTES;
         const int k0 = kb * BN, k1 = k0 + BN - 1;
         const bool cut = it.cut, ids = it.mixed;
-        const int* lid = lid_[buf];
-        arrived();
-        kb = it.next(band, table, nb, lane);
-        buf ^= 1;
-        if (kb >= 0) stage();
+        const int* lid = lids[set][buf];
+        if constexpr (TEAM) arrived_here(); else arrived();
+        if (NB == 2) advance();
         if (rare(cut)) gv.look(lv, largest);
         f32x16 s[NT] = {};
         Rows<T, D> kr;
@@ -803,31 +866,55 @@ __global__ void __launch_bounds__(kThreads, 2) mask_attn_fwd_kernel(const MaskAt
             vc.mma(acc, s[t]);
           }
         }
+        if constexpr (NB == 1) {
+          arrived_here();
+          advance();
+        }
       };
       while (kb >= 0) tile();
       if (rare(met_nonfinite(largest, lbad, seq++))) return false;
       l = sum_halves(l);
-      if (qi < S && h == 0) a.lse[((long)b * a.H + hq) * S + qi] = l == 0.0f ? 0.0f : m + __builtin_log2f(l);
-      store_rows<T, D>((T*)a.out + b * a.so[0] + hq * a.so[1], a.so[2], qw0, S, tiles + wave * 32 * L::RB, acc,
-                       l == 0.0f ? 0.0f : 1.0f / l);
+      float f = 1.0f;
+      if constexpr (TEAM) {
+        if (h == 0) lml[wave][lane] = m, lml[wave][32 + lane] = l;
+        __syncthreads();
+        const int n = lane & 31;
+        const float own_m = m;
+        m = fmaxf(fmaxf(lml[0][n], lml[1][n]), fmaxf(lml[2][n], lml[3][n]));
+        l = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+          l = __builtin_fmaf(lml[i][32 + n], m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(lml[i][n] - m), l);
+        f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(own_m - m);
+      }
+      f = l == 0.0f ? 0.0f : f / l;
+      if (qi < S && h == 0 && (!TEAM || wave == 0))
+        a.lse[((long)b * a.H + hq) * S + qi] = l == 0.0f ? 0.0f : m + __builtin_log2f(l);
+      T* out = (T*)a.out + b * a.so[0] + hq * a.so[1];
+      if constexpr (TEAM)
+        join_rows<T, D>(out, a.so[2], qw0, S, tiles, acc, f);
+      else
+        store_rows<T, D>(out, a.so[2], qw0, S, tiles + wave * 32 * L::RB, acc, f);
       return true;
     };
     if (rare(!item())) {
-      for (int i = qw0; i <= qw1; i++) careful_row<T, D, kForward>(a, b, hq, hk, i);
+      for (int i = qw0 + set; i <= qw1; i += SETS) careful_row<T, D, kForward>(a, b, hq, hk, i);
     }
   }
 }
 
 // ---- backward: dQ, and D_i on the way ---------------------------------------------------------------
-template <typename T, int D, bool PLAIN>
-__global__ void __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) mask_attn_dq_kernel(const MaskAttnArgs a) {
+template <typename T, int D, bool PLAIN, bool TEAM>
+__global__ void __launch_bounds__(kThreads, sizeof(T) == 2 && !TEAM ? 2 : 1) mask_attn_dq_kernel(const MaskAttnArgs a) {
   using L = Tile<T, D>;
-  constexpr int BN = tile_rows<T>(), NT = BN / 32, BM = 128, BYTES = BN * L::RB;
-  __shared__ __align__(1024) char tiles[4 * BYTES];
-  char (*lk_)[BYTES] = (char (*)[BYTES])tiles, (*lv_)[BYTES] = lk_ + 2;
-  __shared__ __align__(16) int lid_[2][64];
+  constexpr int BN = TEAM ? 32 : tile_rows<T>(), NT = BN / 32, BM = TEAM ? 32 : 128, BYTES = BN * L::RB;
+  constexpr int NB = TEAM && L::RB == 512 ? 1 : 2, SETS = TEAM ? 4 : 1;  // buffers, and sets of them
+  __shared__ __align__(1024) char tiles[SETS * 2 * NB * BYTES];
+  __shared__ __align__(16) int lids[SETS][2][64];
   __shared__ int lbad;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5;
+  const int set = TEAM ? wave : 0;
+  char (*lk_)[BYTES] = (char (*)[BYTES])tiles + set * 2 * NB, (*lv_)[BYTES] = lk_ + NB;
   const int S = a.S, nq = (S + BM - 1) / BM, nk = (S + BN - 1) / BN, nb = (S + kTab - 1) / kTab;
   const long total = (long)a.B * a.H * nq;
   const float cs = a.sigma * kLog2e;
@@ -839,25 +926,25 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) mask_attn_dq
   for (long w = blockIdx.x; w < total; w += gridDim.x) {
     const int bh = spread((int)(w % (a.B * a.H)), a.B * a.H), b = bh / a.H, hq = bh % a.H, hk = hq / (a.H / a.Hkv);
     const int q0 = (nq - 1 - (int)(w / (a.B * a.H))) * BM, q1 = min(q0 + BM, S) - 1;
-    const int qw0 = q0 + 32 * wave, qw1 = min(qw0 + 31, S - 1), qi = qw0 + (lane & 31), qr = min(qi, S - 1);
+    const int qw0 = q0 + (TEAM ? 0 : 32 * wave), qw1 = min(qw0 + 31, S - 1), qi = qw0 + (lane & 31), qr = min(qi, S - 1);
     const int* doc = a.doc ? a.doc + (long)b * S : nullptr;
     const i32x4* table = a.doc ? (const i32x4*)a.table + (long)b * nb : nullptr;
     const Band band = {S, a.window, a.prefix ? min(max(a.prefix[b], 0), S) : 0};
     const float slope = !PLAIN && a.slopes ? a.slopes[hq] * kLog2e : 0.0f;
-    Stage<T, D, BN> gk, gv;
+    Stage<T, D, BN, TEAM> gk, gv;
     gk.init((const T*)a.k + b * a.sk[0] + hk * a.sk[1], a.sk[2]);
     gv.init((const T*)a.v + b * a.sv[0] + hk * a.sv[1], a.sv[2]);
 
     const Docs own = docs_of(table, q0 / kTab, q1 / kTab, nb);
     auto item = [&]() {
-      TileIter<BN, true> it;
+      TileIter<BN, true, TEAM> it;
       it.init(q0, q1, own, nk);
       int kb = it.next(band, table, nb, lane), buf = 0;
       Largest<T> largest;  // of cut tiles: with an infinity among them, what is formed here is not used
       auto stage = [&]() {
         gk.copy(lk_[buf], kb * BN, S);
         gv.copy(lv_[buf], kb * BN, S);
-        if (doc && wave == 0) copy_lanes<4>(doc, min(kb * BN + lane, S - 1) * 4, lds_address(lid_[buf]));
+        if (doc && (TEAM || wave == 0)) copy_lanes<4>(doc, min(kb * BN + lane, S - 1) * 4, lds_address(lids[set][buf]));
       };
       __syncthreads();  // the last item is done with LDS
       if (kb >= 0) stage();
@@ -877,21 +964,24 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) mask_attn_dq
         dsum = sum_halves(dsum);
       }
       const long row = ((long)b * a.H + hq) * S + qr;
-      if (qi < S && h == 0) a.dsum[row] = dsum;
+      if (qi < S && h == 0 && (!TEAM || wave == 0)) a.dsum[row] = dsum;
       const float lse = a.lse[row];
       const int qid = doc ? doc[min(qi, S - 1)] : 0;
       f32x16 acc[L::DT] = {};
 
+      auto advance = [&]() {
+        kb = it.next(band, table, nb, lane);
+        buf ^= NB - 1;
+        if (kb >= 0) stage();
+      };
       auto tile = [&]() {
         const char* lk = lk_[buf];
         const uint32_t ak = row_k + buf * BYTES, ac = col_k + buf * BYTES, av = row_v + buf * BYTES;
         const int k0 = kb * BN, k1 = k0 + BN - 1;
         const bool cut = it.cut, ids = it.mixed;
-        const int* lid = lid_[buf];
-        arrived();
-        kb = it.next(band, table, nb, lane);
-        buf ^= 1;
-        if (kb >= 0) stage();
+        const int* lid = lids[set][buf];
+        if constexpr (TEAM) arrived_here(); else arrived();
+        if (NB == 2) advance();
         if (rare(cut)) gk.look(lk, largest);
 #pragma unroll
         for (int t = 0; t < NT; t++) {
@@ -921,14 +1011,22 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) mask_attn_dq
           }
           kc.mma(acc, dp);
         }
+        if constexpr (NB == 1) {
+          arrived_here();
+          advance();
+        }
       };
       while (kb >= 0) tile();
       if (rare(met_nonfinite(largest, lbad, seq++))) return false;
-      store_rows<T, D>((T*)a.dq + b * a.sdq[0] + hq * a.sdq[1], a.sdq[2], qw0, S, tiles + wave * 32 * L::RB, acc, a.sigma);
+      T* out = (T*)a.dq + b * a.sdq[0] + hq * a.sdq[1];
+      if constexpr (TEAM)
+        join_rows<T, D>(out, a.sdq[2], qw0, S, tiles, acc, a.sigma);
+      else
+        store_rows<T, D>(out, a.sdq[2], qw0, S, tiles + wave * 32 * L::RB, acc, a.sigma);
       return true;
     };
     if (rare(!item())) {
-      for (int i = qw0; i <= qw1; i++) careful_row<T, D, kDQ>(a, b, hq, hk, i);
+      for (int i = qw0 + set; i <= qw1; i += SETS) careful_row<T, D, kDQ>(a, b, hq, hk, i);
     }
   }
 }
@@ -936,17 +1034,19 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) mask_attn_dq
 // ---- backward: dK and dV ----------------------------------------------------------------------------
 // SPLIT: a workgroup takes one query head and writes binary32 sums to a.part, which
 // mask_attn_join_kernel adds over the group; otherwise it takes the group's heads one after the other.
-template <typename T, int D, bool PLAIN, bool SPLIT>
-__global__ void __launch_bounds__(kThreads, sizeof(T) * D == 128 ? 2 : 1) mask_attn_dkdv_kernel(const MaskAttnArgs a) {
+template <typename T, int D, bool PLAIN, bool SPLIT, bool TEAM>
+__global__ void __launch_bounds__(kThreads, sizeof(T) * D == 128 && !TEAM ? 2 : 1) mask_attn_dkdv_kernel(const MaskAttnArgs a) {
   using L = Tile<T, D>;
-  constexpr int BN = tile_rows<T>(), NT = BN / 32, BM = 128, BYTES = BN * L::RB;  // BM keys owned, BN queries a tile
+  constexpr int BN = TEAM ? 32 : tile_rows<T>(), NT = BN / 32, BM = TEAM ? 32 : 128, BYTES = BN * L::RB;
+  constexpr int NB = TEAM && L::RB == 512 ? 1 : 2, SETS = TEAM ? 4 : 1;  // buffers, and sets of them  // BM keys owned, BN queries a tile
   constexpr bool PIPELINED = NT == 2 && L::KS == 8 && L::DT == 4;
-  __shared__ __align__(1024) char tiles[4 * BYTES];
-  char (*lq_)[BYTES] = (char (*)[BYTES])tiles, (*lg_)[BYTES] = lq_ + 2;
-  __shared__ __align__(16) float ll_[2][64], ld_[2][64];
-  __shared__ __align__(16) int lid_[2][64];
+  __shared__ __align__(1024) char tiles[SETS * 2 * NB * BYTES];
+  __shared__ __align__(16) float lls[SETS][2][64], lds_[SETS][2][64];
+  __shared__ __align__(16) int lids[SETS][2][64];
   __shared__ int lbad;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5;
+  const int set = TEAM ? wave : 0;
+  char (*lq_)[BYTES] = (char (*)[BYTES])tiles + set * 2 * NB, (*lg_)[BYTES] = lq_ + NB;
   const int S = a.S, nkb = (S + BM - 1) / BM, nq = (S + BN - 1) / BN, nb = (S + kTab - 1) / kTab;
   const int group = a.H / a.Hkv, heads = SPLIT ? a.H : a.Hkv;
   const long total = (long)a.B * heads * nkb;
@@ -960,7 +1060,7 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) * D == 128 ? 2 : 1) mask_a
     // the first keys have the most queries, so they come first
     const int bh = (int)(w % ((long)a.B * heads)), b = bh / heads, head = bh % heads, hk = SPLIT ? head / group : head;
     const int k0 = (int)(w / ((long)a.B * heads)) * BM, k1 = min(k0 + BM, S) - 1;
-    const int kw0 = k0 + 32 * wave, kw1 = min(kw0 + 31, S - 1), kj = kw0 + (lane & 31), kr = min(kj, S - 1);
+    const int kw0 = k0 + (TEAM ? 0 : 32 * wave), kw1 = min(kw0 + 31, S - 1), kj = kw0 + (lane & 31), kr = min(kj, S - 1);
     const int* doc = a.doc ? a.doc + (long)b * S : nullptr;
     const i32x4* table = a.doc ? (const i32x4*)a.table + (long)b * nb : nullptr;
     const Band band = {S, a.window, a.prefix ? min(max(a.prefix[b], 0), S) : 0};
@@ -971,50 +1071,57 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) * D == 128 ? 2 : 1) mask_a
       f32x16 dk[L::DT] = {}, dv[L::DT] = {};
       Largest<T> largest;
       int hq = first, buf = 0;  // the head whose queries are copied next
-      Stage<T, D, BN> gq, gg;
+      Stage<T, D, BN, TEAM> gq, gg;
       auto take_head = [&]() {
         gq.init((const T*)a.q + b * a.sq[0] + hq * a.sq[1], a.sq[2]);
         gg.init((const T*)a.dout + b * a.sdo[0] + hq * a.sdo[1], a.sdo[2]);
       };
-      TileIter<BN, false> it;
+      TileIter<BN, false, TEAM> it;
       it.init(k0, k1, own, nq);
-      int qb = it.next(band, table, nb, lane);
+      int qb;
+      auto seek = [&]() {  // the next tile, of this head or of the one after it
+        qb = it.next(band, table, nb, lane);
+        if (qb < 0 && hq + 1 < last) {  // a team has one head
+          hq++;
+          take_head();
+          it.again();
+          qb = it.next(band, table, nb, lane);
+        }
+      };
       auto stage = [&]() {
         gq.copy(lq_[buf], qb * BN, S);
         gg.copy(lg_[buf], qb * BN, S);
         const int i = min(qb * BN + lane, S - 1) * 4;  // 64 rows, BN of them read
         const long row0 = ((long)b * a.H + hq) * S;
-        if (wave == 0) copy_lanes<4>(a.lse + row0, i, lds_address(ll_[buf]));
-        if (wave == 1) copy_lanes<4>(a.dsum + row0, i, lds_address(ld_[buf]));
-        if (doc && wave == 2) copy_lanes<4>(doc, i, lds_address(lid_[buf]));
+        if (TEAM || wave == 0) copy_lanes<4>(a.lse + row0, i, lds_address(lls[set][buf]));
+        if (TEAM || wave == 1) copy_lanes<4>(a.dsum + row0, i, lds_address(lds_[set][buf]));
+        if (doc && (TEAM || wave == 2)) copy_lanes<4>(doc, i, lds_address(lids[set][buf]));
       };
       __syncthreads();  // the last item is done with LDS
       take_head();
+      seek();
       if (qb >= 0) stage();
       u32x4 kf[L::KS], vf[L::KS];
       load_own<T, D>(kf, (const T*)a.k + b * a.sk[0] + hk * a.sk[1], a.sk[2], kr, lane);
       load_own<T, D>(vf, (const T*)a.v + b * a.sv[0] + hk * a.sv[1], a.sv[2], kr, lane);
       const int kid = doc ? doc[kr] : 0;
 
+      auto advance = [&]() {
+        seek();
+        buf ^= NB - 1;
+        if (qb >= 0) stage();
+      };
       auto tile = [&](auto masks) {
       constexpr bool MASKED = decltype(masks)::value;
         const char *lq = lq_[buf], *lg = lg_[buf];
-        const float *ll = ll_[buf], *ld = ld_[buf];
+        const float *ll = lls[set][buf], *ld = lds_[set][buf];
         const uint32_t off = buf * BYTES;
         const int q0 = qb * BN, q1 = q0 + BN - 1;
         const bool cut = it.cut, ids = it.mixed;
-        const int* lid = lid_[buf];
+        const int* lid = lids[set][buf];
         const float slope = !PLAIN && a.slopes ? a.slopes[hq] * kLog2e : 0.0f;
-        arrived();
-        qb = it.next(band, table, nb, lane);
-        if (qb < 0 && hq + 1 < last) {
-          hq++;
-          take_head();
-          it.again();
-          qb = it.next(band, table, nb, lane);
-        }
-        buf ^= 1;
-        if (qb >= 0) stage();
+        if constexpr (TEAM) arrived_here(); else arrived();
+        if (NB == 2) advance();
         if (MASKED && rare(cut)) {
           gq.look(lq, largest);
           gg.look(lg, largest);
@@ -1106,6 +1213,10 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) * D == 128 ? 2 : 1) mask_a
             qc.mma(dk, dp[t]);
           }
         }
+        if constexpr (NB == 1) {
+          arrived_here();
+          advance();
+        }
       };
       while (qb >= 0) {
         if constexpr (PIPELINED)
@@ -1113,20 +1224,26 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) * D == 128 ? 2 : 1) mask_a
         while (qb >= 0 && (it.cut || !PIPELINED)) tile(std::true_type());
       }
       if (rare(met_nonfinite(largest, lbad, seq++))) return false;
+      auto put = [&](auto* dk_at, long dk_stride, auto* dv_at, long dv_stride) {
+        if constexpr (TEAM) {
+          join_rows<T, D>(dk_at, dk_stride, kw0, S, tiles, dk, a.sigma);
+          join_rows<T, D>(dv_at, dv_stride, kw0, S, tiles, dv, 1.0f);
+        } else {
+          char* lds = tiles + wave * 32 * D * (int)sizeof(*dk_at);
+          store_rows<T, D>(dk_at, dk_stride, kw0, S, lds, dk, a.sigma);
+          store_rows<T, D>(dv_at, dv_stride, kw0, S, lds, dv, 1.0f);
+        }
+      };
       if constexpr (SPLIT) {
         float* p = a.part + ((long)b * a.H + first) * S * D;
-        char* lds = tiles + wave * 32 * 4 * D;
-        store_rows<T, D>(p, D, kw0, S, lds, dk, a.sigma);
-        store_rows<T, D>(p + (long)a.B * a.H * S * D, D, kw0, S, lds, dv, 1.0f);
+        put(p, D, p + (long)a.B * a.H * S * D, D);
       } else {
-        char* lds = tiles + wave * 32 * L::RB;
-        store_rows<T, D>((T*)a.dk + b * a.sdk[0] + hk * a.sdk[1], a.sdk[2], kw0, S, lds, dk, a.sigma);
-        store_rows<T, D>((T*)a.dv + b * a.sdv[0] + hk * a.sdv[1], a.sdv[2], kw0, S, lds, dv, 1.0f);
+        put((T*)a.dk + b * a.sdk[0] + hk * a.sdk[1], a.sdk[2], (T*)a.dv + b * a.sdv[0] + hk * a.sdv[1], a.sdv[2]);
       }
       return true;
     };
     if (rare(!item())) {
-      for (int j = kw0; j <= kw1; j++) careful_row<T, D, SPLIT ? kDKDVPart : kDKDV>(a, b, first, hk, j);
+      for (int j = kw0 + set; j <= kw1; j += SETS) careful_row<T, D, SPLIT ? kDKDVPart : kDKDV>(a, b, first, hk, j);
     }
   }
 }
@@ -1171,21 +1288,47 @@ hipError_t launch_mask_table(const int* doc, void* table, int B, int S, hipStrea
   return hipGetLastError();
 }
 
+// Whether the work is too little for the device in blocks of 128 rows: then a team of four waves takes 32
+// rows, with tiles and sums of its own in each wave.  The waves share no tile, so this moves four times
+// the data a row, and pays while compute units would stand idle, and from the third tile on.  Forward, dQ
+// and dK/dV in us, blocks and teams: 2 x 4 heads x 197 binary32 28, 38, 49 and 14, 19, 21; 16 heads x 512
+// bf16 (64 blocks) 18, 25, 28 and 14, 18, 18; 2 heads x 8192 (128 blocks) 123, 158, 214 and 64, 76, 108;
+// 16 x 2048 (256 blocks) 49, 66, 80 and 70, 85, 95; 4 x 8 x 1000 binary32 (256) 86, 125, 165 and 75, 101, 120;
+// 8 heads x 64 bf16, one tile, 8, 11, 11 and 9, 11, 11.
+template <typename T>
+static bool team_of(int B, int heads, int S) {
+  const long blocks = (long)B * heads * ((S + 127) / 128);
+  return S > 2 * tile_rows<T>() && blocks * (sizeof(T) == 2 ? 2 : 1) <= otx_cu_count();
+}
+
 template <typename T, int D, bool PLAIN>
 static hipError_t fwd_of(const MaskAttnArgs& a, hipStream_t st) {
-  mask_attn_fwd_kernel<T, D, PLAIN><<<grid_of((long)a.B * a.H * ((a.S + 127) / 128)), kThreads, 0, st>>>(a);
+  if (team_of<T>(a.B, a.H, a.S))
+    mask_attn_fwd_kernel<T, D, PLAIN, true><<<grid_of((long)a.B * a.H * ((a.S + 31) / 32)), kThreads, 0, st>>>(a);
+  else
+    mask_attn_fwd_kernel<T, D, PLAIN, false><<<grid_of((long)a.B * a.H * ((a.S + 127) / 128)), kThreads, 0, st>>>(a);
   return hipGetLastError();
+}
+
+template <typename T, int D, bool PLAIN, bool SPLIT>
+static void dkdv_of(const MaskAttnArgs& a, int heads, hipStream_t st) {
+  if (team_of<T>(a.B, heads, a.S))
+    mask_attn_dkdv_kernel<T, D, PLAIN, SPLIT, true><<<grid_of((long)a.B * heads * ((a.S + 31) / 32)), kThreads, 0, st>>>(a);
+  else
+    mask_attn_dkdv_kernel<T, D, PLAIN, SPLIT, false><<<grid_of((long)a.B * heads * ((a.S + 127) / 128)), kThreads, 0, st>>>(a);
 }
 
 template <typename T, int D, bool PLAIN>
 static hipError_t bwd_of(const MaskAttnArgs& a, hipStream_t st) {
-  const long nt = (a.S + 127) / 128;
-  mask_attn_dq_kernel<T, D, PLAIN><<<grid_of((long)a.B * a.H * nt), kThreads, 0, st>>>(a);
+  if (team_of<T>(a.B, a.H, a.S))
+    mask_attn_dq_kernel<T, D, PLAIN, true><<<grid_of((long)a.B * a.H * ((a.S + 31) / 32)), kThreads, 0, st>>>(a);
+  else
+    mask_attn_dq_kernel<T, D, PLAIN, false><<<grid_of((long)a.B * a.H * ((a.S + 127) / 128)), kThreads, 0, st>>>(a);
   if (a.part) {
-    mask_attn_dkdv_kernel<T, D, PLAIN, true><<<grid_of((long)a.B * a.H * nt), kThreads, 0, st>>>(a);
+    dkdv_of<T, D, PLAIN, true>(a, a.H, st);
     mask_attn_join_kernel<T, D><<<grid_of(((long)a.B * a.Hkv * a.S * (D / 2) + 255) / 256), 256, 0, st>>>(a);
   } else {
-    mask_attn_dkdv_kernel<T, D, PLAIN, false><<<grid_of((long)a.B * a.Hkv * nt), kThreads, 0, st>>>(a);
+    dkdv_of<T, D, PLAIN, false>(a, a.Hkv, st);
   }
   return hipGetLastError();
 }

@@ -92,6 +92,26 @@ def test_against_binary64(dtype, B, H, Hkv, S, D, window, cap, alibi, docs, pref
     assert (got[0].cpu()[empty] == 0).all() and (got[1].cpu()[empty] == 0).all()
 
 
+@pytest.mark.parametrize("heads", [1, 8])
+@pytest.mark.parametrize("dtype,B,H,Hkv,S,D,window,cap,alibi,docs,prefix", [c for c in CASES if c[4] > 64])
+def test_full_grids_against_binary64(dtype, B, H, Hkv, S, D, window, cap, alibi, docs, prefix, heads):
+    """The same rows many times over, so that blocks of 128 rows fill the device: a workgroup's waves share their tiles
+    (in CASES, from S = 129, they do not), and with many key/value heads dK/dV walks a group's heads in one.  One repetition
+    against binary64, the others against it bit for bit."""
+    H, Hkv = H * heads, Hkv * heads
+    n = -(-520 // (B * Hkv * -(-S // 128))) if heads > 1 else -(-260 // (B * H * -(-S // 128)))
+    (q, k, v, do), gen = make(B, H, Hkv, S, D, dtype)
+    doc = docs_of(docs, B, S, gen)
+    slopes = 2.0 ** -(torch.arange(H, dtype=F32) / heads + 1) if alibi else None
+    pre = torch.tensor([(S * (b + 1)) // (B + 2) for b in range(B)], dtype=torch.int32) if prefix else None
+    over = [t if t is None else torch.cat([t] * n) for t in (q, k, v, do, doc, pre)]
+    got = run(*over[:4], window=window, softcap=cap, slopes=slopes, doc_ids=over[4], prefix=over[5])
+    for x in got:
+        for i in range(1, n):
+            assert torch.equal(x[i * B:(i + 1) * B], x[:B])
+    compare([x[:B] for x in got], reference(q, k, v, do, visible(S, window, doc, pre), cap, slopes, dtype))
+
+
 @pytest.mark.parametrize("dtype", [BF, F32])
 def test_large_scores(dtype):
     """Maxima that move by far more than the threshold of the running rescale, in both directions."""
