@@ -1277,9 +1277,14 @@ int grid_of(long work) { return (int)(work < (1 << 20) ? work : (1 << 20)); }
 
 }  // namespace
 
-// Whether dK/dV splits a group of query heads over workgroups.
-bool mask_attn_splits(int B, int H, int Hkv, int S) {
-  return H > Hkv && (long)B * Hkv * ((S + 127) / 128) < 2 * otx_cu_count();
+// Whether dK/dV splits a group of query heads over workgroups: that evens out what the compute units get,
+// which counts with few blocks, with long sequences (the first keys have the most queries) and with
+// documents (of unequal lengths), and costs the partial sums.  Groups of four heads of 128 bf16 columns,
+// whole and split, in us: 128 blocks of 1024 tokens 232 and 79, 256 of 1024 152 and 156, 256 of 4096 563
+// and 374, 512 of 1024 201 and 327, of 4096 660 and 731; with documents of 500 tokens 541 and 385.
+bool mask_attn_splits(int B, int H, int Hkv, int S, bool documents) {
+  const long blocks = (long)B * Hkv * ((S + 127) / 128);
+  return H > Hkv && blocks < (documents ? 3 : S >= 2048 ? 2 : 1) * otx_cu_count();
 }
 
 hipError_t launch_mask_table(const int* doc, void* table, int B, int S, hipStream_t st) {

@@ -469,7 +469,7 @@ struct MaskedAttention : Function<MaskedAttention> {
     std::vector<long> st;
     for (const Tensor& t : {q, k, v, o, dout, dq, dk, dv}) put_strides(st, t);
     Launch at(q);
-    const size_t nbytes = otx_mask_attn_bwd_workspace_bytes((int)B, (int)H, (int)Hkv, (int)S, (int)D);
+    const size_t nbytes = otx_mask_attn_bwd_workspace_bytes((int)B, (int)H, (int)Hkv, (int)S, (int)D, (has & 4) != 0);
     const Workspace ws(q, nbytes);
     check(otx_mask_attn_bwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), lse.data_ptr<float>(),
                             dout.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),

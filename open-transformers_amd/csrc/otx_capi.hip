@@ -47,7 +47,7 @@ hipError_t launch_swiglu(int dtype, int backward, const void* gu, const void* dh
 hipError_t launch_rope_heads(int dtype, int backward, const void* in, const float* cosv, const float* sinv, void* out,
                              int B, int Tn, int H, int D, hipStream_t st);
 hipError_t launch_swap_heads(int dtype, const void* in, void* out, int B, int X, int Y, int D, hipStream_t st);
-bool mask_attn_splits(int B, int H, int Hkv, int S);
+bool mask_attn_splits(int B, int H, int Hkv, int S, bool documents);
 hipError_t launch_mask_table(const int* doc, void* table, int B, int S, hipStream_t st);
 hipError_t launch_mask_attn(int dtype, int D, bool backward, const MaskAttnArgs& a, hipStream_t st);
 hipError_t launch_rotary(int dtype, const RotaryArgs& a, bool half, hipStream_t st);
@@ -839,9 +839,9 @@ size_t otx_mask_attn_table_bytes(int B, int S) {
 
 static size_t mask_dsum_bytes(int B, int H, int S) { return ((size_t)B * H * S * 4 + 255) / 256 * 256; }
 
-size_t otx_mask_attn_bwd_workspace_bytes(int B, int H, int Hkv, int S, int D) {
+size_t otx_mask_attn_bwd_workspace_bytes(int B, int H, int Hkv, int S, int D, int documents) {
   if (check_mask_shape(B, H, Hkv, S, D) != OTX_OK) return 0;
-  return mask_dsum_bytes(B, H, S) + (otx::mask_attn_splits(B, H, Hkv, S) ? (size_t)B * H * S * D * 8 : 0);
+  return mask_dsum_bytes(B, H, S) + (otx::mask_attn_splits(B, H, Hkv, S, documents != 0) ? (size_t)B * H * S * D * 8 : 0);
 }
 
 int otx_mask_attn_fwd(const void* q, const void* k, const void* v, void* o, float* lse, const float* slopes,
@@ -876,12 +876,12 @@ int otx_mask_attn_bwd(const void* q, const void* k, const void* v, const void* o
       (rc = mask_strides("dv", dv, strides + 21, dtype, a.sdv)))
     return rc;
   if ((uintptr_t)workspace & 255u) return fail(OTX_EINVAL, "the workspace must be 256-byte aligned");
-  const size_t need = otx_mask_attn_bwd_workspace_bytes(B, H, Hkv, S, D);
+  const size_t need = otx_mask_attn_bwd_workspace_bytes(B, H, Hkv, S, D, doc_ids != nullptr);
   if (workspace_bytes < need)
     return fail(OTX_EINVAL, "workspace too small: %zu bytes given, %zu needed", workspace_bytes, need);
   a.q = q, a.k = k, a.v = v, a.o = o, a.lse = (float*)lse, a.dout = dout, a.dq = dq, a.dk = dk, a.dv = dv;
   a.dsum = (float*)workspace;
-  if (otx::mask_attn_splits(B, H, Hkv, S)) a.part = (float*)((char*)workspace + mask_dsum_bytes(B, H, S));
+  if (otx::mask_attn_splits(B, H, Hkv, S, doc_ids != nullptr)) a.part = (float*)((char*)workspace + mask_dsum_bytes(B, H, S));
   hipError_t e = otx::launch_mask_attn(dtype, D, true, a, (hipStream_t)stream);
   return e == hipSuccess ? OTX_OK : fail(OTX_EHIP, "masked attention backward launch failed: %s", hipGetErrorString(e));
 }

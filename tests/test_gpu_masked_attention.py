@@ -99,7 +99,7 @@ def test_full_grids_against_binary64(dtype, B, H, Hkv, S, D, window, cap, alibi,
     (in CASES, from S = 129, they do not), and with many key/value heads dK/dV walks a group's heads in one.  One repetition
     against binary64, the others against it bit for bit."""
     H, Hkv = H * heads, Hkv * heads
-    n = -(-520 // (B * Hkv * -(-S // 128))) if heads > 1 else -(-260 // (B * H * -(-S // 128)))
+    n = -(-780 // (B * Hkv * -(-S // 128))) if heads > 1 else -(-260 // (B * H * -(-S // 128)))
     (q, k, v, do), gen = make(B, H, Hkv, S, D, dtype)
     doc = docs_of(docs, B, S, gen)
     slopes = 2.0 ** -(torch.arange(H, dtype=F32) / heads + 1) if alibi else None
