@@ -284,18 +284,20 @@ int otx_swap_heads(const void* x, void* y, int B, int X, int Y, int D, int dtype
  * contiguous, rows start at 16-byte boundaries.  slopes float32 [H], doc_ids
  * int32 [B, S], prefix int32 [B].  table: otx_mask_attn_table_bytes(B, S), written
  * by the forward where doc_ids are given and read by the backward.  documents:
- * whether the backward gets doc_ids.  lse
+ * whether the backward gets doc_ids.  o_low: B H S D bytes of the forward for the
+ * backward, 16-byte aligned, the bits of bf16 outputs past their rounding; NULL
+ * where no backward follows, or for one that takes o as it is.  lse
  * float32 [B, H, S], as the forward leaves it (units of log 2).
  * These operators are not under the contract above: products run on the bf16
  * matrix units with P and dS rounded to bf16 (binary32 tensors: on the binary32
  * ones), sums and softmax statistics are binary32.  Results repeat bit for bit. */
 size_t otx_mask_attn_table_bytes(int B, int S);
 size_t otx_mask_attn_bwd_workspace_bytes(int B, int H, int Hkv, int S, int D, int documents);
-int otx_mask_attn_fwd(const void* q, const void* k, const void* v, void* o, float* lse, const float* slopes,
+int otx_mask_attn_fwd(const void* q, const void* k, const void* v, void* o, void* o_low, float* lse, const float* slopes,
                       const int32_t* doc_ids, const int32_t* prefix, void* table, const long* strides, int B, int H,
                       int Hkv, int S, int D, int window, float softcap, int dtype, void* stream);
-int otx_mask_attn_bwd(const void* q, const void* k, const void* v, const void* o, const float* lse, const void* dout,
-                      void* dq, void* dk, void* dv, const float* slopes, const int32_t* doc_ids, const int32_t* prefix,
+int otx_mask_attn_bwd(const void* q, const void* k, const void* v, const void* o, const void* o_low, const float* lse,
+                      const void* dout, void* dq, void* dk, void* dv, const float* slopes, const int32_t* doc_ids, const int32_t* prefix,
                       const void* table, const long* strides, int B, int H, int Hkv, int S, int D, int window,
                       float softcap, int dtype, void* workspace, size_t workspace_bytes, void* stream);
 

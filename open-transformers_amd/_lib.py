@@ -64,8 +64,8 @@ _SIGNATURES = {
     "otx_swap_heads": (_i, [_vp, _vp, _i, _i, _i, _i, _i, _vp]),
     "otx_mask_attn_table_bytes": (_sz, [_i, _i]),
     "otx_mask_attn_bwd_workspace_bytes": (_sz, [_i] * 6),
-    "otx_mask_attn_fwd": (_i, [_vp] * 10 + [_i] * 6 + [ctypes.c_float, _i, _vp]),
-    "otx_mask_attn_bwd": (_i, [_vp] * 14 + [_i] * 6 + [ctypes.c_float, _i, _vp, _sz, _vp]),
+    "otx_mask_attn_fwd": (_i, [_vp] * 11 + [_i] * 6 + [ctypes.c_float, _i, _vp]),
+    "otx_mask_attn_bwd": (_i, [_vp] * 15 + [_i] * 6 + [ctypes.c_float, _i, _vp, _sz, _vp]),
     "otx_rotary": (_i, [_vp] * 6 + [_i] * 9 + [_vp]),
     "otx_layer_norm_fwd": (_i, [_vp] * 6 + [_l, _i, ctypes.c_float, _i, _vp]),
     "otx_layer_norm_bwd_workspace_bytes": (_sz, [_l, _i]),

@@ -24,6 +24,11 @@
 // and the A operand is read from LDS with the same permutation (transposing reads,
 // ds_read_b64_tr_b16, for bf16).  P and dS never pass through LDS.
 //
+// D_i is formed from O with eight more bits than its bf16 holds, which the forward keeps where a gradient
+// will be wanted: rounded to bf16, O would alone cost gradients of 2^-8 relative where rows see few keys
+// (documents of two tokens, dQ: 0.0036 of its norm off binary64 instead of 0.0026, of which 0.0017 is the
+// rounding of the result), and a byte an element is what it takes.
+//
 // Masked pairs contribute nothing, whatever their rows hold.  A weight of 0 times a NaN or an
 // infinity is NaN, so a tile that some rows of the workgroup do not see whole is checked for
 // non-finite values, and a workgroup that finds one does its rows over, one at a time
@@ -479,12 +484,19 @@ __device__ __forceinline__ void load_own(u32x4 (&f)[D * sizeof(T) / 32], const T
     f[ks] = *(const u32x4*)(base + (long)row * stride + (2 * ks + (lane >> 5)) * (16 / (int)sizeof(T)));
 }
 
+// The eight bits of x after those that its bf16 rounding keeps, signed.
+__device__ __forceinline__ int low_bits(float x) {
+  const uint32_t high = (uint32_t)Elem<uint16_t>::put(x) << 16;
+  return min((int)(__float_as_uint(x) - high) >> 8, 127);
+}
+__device__ __forceinline__ float with_low(float high, int low) { return __uint_as_float(__float_as_uint(high) + ((uint32_t)low << 8)); }
+
 // Writes the 32 rows of a wave: acc^T (column n: row n) times f, to row * stride.  The results pass
 // through this wave's share of LDS, so that 16 bytes a lane go to whole rows: stored as the lanes hold
 // them, 8 bytes to each of 32 rows, they took 3 us of a workgroup's time.
 template <typename T, int D, typename O>
 __device__ __forceinline__ void store_rows(O* out, long stride, int row0, int S, char* lds, const f32x16 (&acc)[D / 32],
-                                           float f) {
+                                           float f, signed char* low = nullptr) {
   const int lane = here(threadIdx.x) & 63;
   constexpr int E = 16 / (int)sizeof(O), C = D / E;  // elements of a chunk, chunks of a row
   const int n = lane & 31, h = lane >> 5;
@@ -512,12 +524,30 @@ __device__ __forceinline__ void store_rows(O* out, long stride, int row0, int S,
     const u32x4 v = *(const u32x4*)(lds + r * D * (int)sizeof(O) + ((c ^ (r & (C - 1) & 15)) << 4));
     if (row0 + r < S) *(u32x4*)(out + (row0 + r) * stride + c * E) = v;
   }
+  if (sizeof(O) == 2 && low) {
+    constexpr int CL = D / 16;
+#pragma unroll
+    for (int dt = 0; dt < D / 32; dt++)
+#pragma unroll
+      for (int g = 0; g < 4; g++) {
+        uint32_t w = 0;
+#pragma unroll
+        for (int i = 0; i < 4; i++) w |= (uint32_t)(low_bits(acc[dt][4 * g + i] * f) & 255) << (8 * i);
+        *(uint32_t*)(lds + n * D + (((2 * dt + g / 2) ^ (n & (CL - 1))) << 4) + 8 * (g & 1) + 4 * h) = w;
+      }
+#pragma unroll
+    for (int i = 0; i < CL / 2; i++) {
+      const int r = (i * 64 + lane) / CL, c = (i * 64 + lane) % CL;
+      const u32x4 v = *(const u32x4*)(lds + r * D + ((c ^ (r & (CL - 1))) << 4));
+      if (row0 + r < S) *(u32x4*)(low + (long)(row0 + r) * D + c * 16) = v;
+    }
+  }
 }
 
 // The same for a team, whose four waves hold summands of the same 32 rows: added in the waves' order.
 template <typename T, int D, typename O>
 __device__ __forceinline__ void join_rows(O* out, long stride, int row0, int S, char* lds, const f32x16 (&acc)[D / 32],
-                                          float f) {
+                                          float f, signed char* low = nullptr) {
   constexpr int C = D / 4, PART = 32 * D * 4;  // chunks of four columns in a row, bytes of a wave's summand
   const int tid = here(threadIdx.x), lane = tid & 63, n = lane & 31, h = lane >> 5;
   char* mine = lds + (tid >> 6) * PART;
@@ -547,6 +577,12 @@ __device__ __forceinline__ void join_rows(O* out, long stride, int row0, int S, 
 #pragma unroll
         for (int e = 0; e < 4; e++) v[e] = (__bf16)o[e];
         *(bf16x4*)to = v;
+        if (low) {
+          uint32_t l = 0;
+#pragma unroll
+          for (int e = 0; e < 4; e++) l |= (uint32_t)(low_bits(o[e]) & 255) << (8 * e);
+          *(uint32_t*)(low + (long)(row0 + r) * D + c * 4) = l;
+        }
       } else {
         *(f32x4*)to = o;
       }
@@ -689,7 +725,9 @@ __device__ __forceinline__ void careful_row(const MaskAttnArgs& a, int b, int he
   for (int c = 0; c < C; c++) {
     const int d = lane + 64 * c;
     if constexpr (WHAT == kForward) {
-      ((T*)a.out)[b * a.so[0] + head * a.so[1] + own * a.so[2] + d] = Elem<T>::put(l == 0.0f ? 0.0f : x[c] / l);
+      const float o = l == 0.0f ? 0.0f : x[c] / l;
+      ((T*)a.out)[b * a.so[0] + head * a.so[1] + own * a.so[2] + d] = Elem<T>::put(o);
+      if (a.low) a.low[row * D + d] = (signed char)low_bits(o);
     } else if constexpr (WHAT == kDQ) {
       ((T*)a.dq)[b * a.sdq[0] + head * a.sdq[1] + own * a.sdq[2] + d] = Elem<T>::put(x[c] * a.sigma);
     } else if constexpr (WHAT == kDKDVPart) {
@@ -891,10 +929,11 @@ __global__ void __launch_bounds__(kThreads, TEAM || sizeof(T) * D == 512 ? 1 : 2
       if (qi < S && h == 0 && (!TEAM || wave == 0))
         a.lse[((long)b * a.H + hq) * S + qi] = l == 0.0f ? 0.0f : m + __builtin_log2f(l);
       T* out = (T*)a.out + b * a.so[0] + hq * a.so[1];
+      signed char* low = a.low ? a.low + ((long)b * a.H + hq) * S * D : nullptr;
       if constexpr (TEAM)
-        join_rows<T, D>(out, a.so[2], qw0, S, tiles, acc, f);
+        join_rows<T, D>(out, a.so[2], qw0, S, tiles, acc, f, low);
       else
-        store_rows<T, D>(out, a.so[2], qw0, S, tiles + wave * 32 * L::RB, acc, f);
+        store_rows<T, D>(out, a.so[2], qw0, S, tiles + wave * 32 * L::RB, acc, f, low);
       return true;
     };
     if (rare(!item())) {
@@ -951,19 +990,24 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 2 && !TEAM ? 2 : 1) mas
       u32x4 qf[L::KS], gf[L::KS];
       load_own<T, D>(qf, (const T*)a.q + b * a.sq[0] + hq * a.sq[1], a.sq[2], qr, lane);
       load_own<T, D>(gf, (const T*)a.dout + b * a.sdo[0] + hq * a.sdo[1], a.sdo[2], qr, lane);
+      const long row = ((long)b * a.H + hq) * S + qr;
       float dsum = 0.0f;
       {
         const T* op = (const T*)a.o + b * a.so[0] + hq * a.so[1] + qr * a.so[2];
 #pragma unroll
         for (int ks = 0; ks < L::KS; ks++) {
           const u32x4 of = *(const u32x4*)(op + (2 * ks + h) * (16 / (int)sizeof(T)));
+          uint2 low = make_uint2(0, 0);
+          if (sizeof(T) == 2 && a.low) low = *(const uint2*)(a.low + row * D + (2 * ks + h) * 8);
 #pragma unroll
-          for (int e = 0; e < Elem<T>::VEC; e++)
-            dsum = __builtin_fmaf(element<T>(gf[ks], e), element<T>(of, e), dsum);
+          for (int e = 0; e < Elem<T>::VEC; e++) {
+            float x = element<T>(of, e);
+            if constexpr (sizeof(T) == 2) x = with_low(x, (int)((e < 4 ? low.x : low.y) << (24 - 8 * (e & 3))) >> 24);
+            dsum = __builtin_fmaf(element<T>(gf[ks], e), x, dsum);
+          }
         }
         dsum = sum_halves(dsum);
       }
-      const long row = ((long)b * a.H + hq) * S + qr;
       if (qi < S && h == 0 && (!TEAM || wave == 0)) a.dsum[row] = dsum;
       const float lse = a.lse[row];
       const int qid = doc ? doc[min(qi, S - 1)] : 0;

@@ -7,6 +7,7 @@ struct MaskAttnArgs {
   const void *q, *k, *v, *o, *dout;
   void *out, *dq, *dk, *dv;
   float *lse, *dsum;    // [B, H, S]; lse in units of log 2
+  signed char* low;     // [B, H, S, D] or null: the next eight bits of O's significands
   float* part;          // dK/dV partial sums of each query head, [2][B, H, S, D], or null
   const float* slopes;  // [H] or null
   const int* doc;       // [B, S] or null

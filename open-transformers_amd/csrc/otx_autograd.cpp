@@ -412,31 +412,35 @@ Tensor empty_rows(const Tensor& t) {
 struct MaskedAttention : Function<MaskedAttention> {
   static Tensor forward(AutogradContext* ctx, const Tensor& q_, const Tensor& k_, const Tensor& v_,
                         const std::optional<Tensor>& slopes, const std::optional<Tensor>& doc,
-                        const std::optional<Tensor>& prefix, int64_t window, double softcap) {
+                        const std::optional<Tensor>& prefix, int64_t window, double softcap, bool grad) {
     const Tensor q = rows16(q_), k = rows16(k_), v = rows16(v_);
     const int B = (int)q.size(0), H = (int)q.size(1), Hkv = (int)k.size(1), S = (int)q.size(2), D = (int)q.size(3);
     // in q's order of dimensions, so that the heads of a [B, S, H, D] projection merge without a copy
     const Tensor o = empty_rows(q), lse = at::empty({B, H, S}, q.options().dtype(at::kFloat));
     const Tensor table =
         doc ? at::empty({(int64_t)otx_mask_attn_table_bytes(B, S) / 4}, q.options().dtype(at::kInt)) : Tensor();
+    const bool keep = grad && q.scalar_type() == at::kBFloat16;
+    const Tensor low = keep ? at::empty({B, H, S, D}, q.options().dtype(at::kChar)) : Tensor();
     std::vector<long> st;
     for (const Tensor& t : {q, k, v, o}) put_strides(st, t);
     {
       Launch at(q);
-      check(otx_mask_attn_fwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), lse.data_ptr<float>(),
+      check(otx_mask_attn_fwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(),
+                              keep ? low.data_ptr() : nullptr, lse.data_ptr<float>(),
                               slopes ? slopes->data_ptr<float>() : nullptr, doc ? doc->data_ptr<int>() : nullptr,
                               prefix ? prefix->data_ptr<int>() : nullptr, doc ? table.data_ptr() : nullptr, st.data(),
                               B, H, Hkv, S, D, (int)window, (float)softcap, dtype_code(q), at.stream),
             "otx_mask_attn_fwd");
     }
     variable_list save = {q, k, v, o, lse};
+    if (keep) save.push_back(low);
     if (slopes) save.push_back(*slopes);
     if (prefix) save.push_back(*prefix);
     if (doc) save.push_back(*doc), save.push_back(table);
     ctx->save_for_backward(save);
     ctx->saved_data["window"] = window;
     ctx->saved_data["softcap"] = softcap;
-    ctx->saved_data["has"] = (int64_t)((slopes ? 1 : 0) | (prefix ? 2 : 0) | (doc ? 4 : 0));
+    ctx->saved_data["has"] = (int64_t)((slopes ? 1 : 0) | (prefix ? 2 : 0) | (doc ? 4 : 0) | (keep ? 8 : 0));
     return o;
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
@@ -457,7 +461,8 @@ struct MaskedAttention : Function<MaskedAttention> {
                  v = strided(saved[2], {B, Hkv, S, D}, "v"), o = strided(saved[3], {B, H, S, D}, "o");
     const Tensor lse = saved_as(saved[4], {B, H, S}, at::kFloat, dout, "masked_attention: the logsumexp");
     size_t at_ = 5;
-    Tensor slopes, prefix, doc, table;
+    Tensor low, slopes, prefix, doc, table;
+    if (has & 8) low = saved_as(saved[at_++], {B, H, S, D}, at::kChar, dout, "masked_attention: the low bits of o");
     if (has & 1) slopes = saved_as(saved[at_++], {H}, at::kFloat, dout, "masked_attention: slopes");
     if (has & 2) prefix = saved_as(saved[at_++], {B}, at::kInt, dout, "masked_attention: prefix");
     if (has & 4) {
@@ -471,14 +476,14 @@ struct MaskedAttention : Function<MaskedAttention> {
     Launch at(q);
     const size_t nbytes = otx_mask_attn_bwd_workspace_bytes((int)B, (int)H, (int)Hkv, (int)S, (int)D, (has & 4) != 0);
     const Workspace ws(q, nbytes);
-    check(otx_mask_attn_bwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), lse.data_ptr<float>(),
-                            dout.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
+    check(otx_mask_attn_bwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(),
+                            has & 8 ? low.data_ptr() : nullptr, lse.data_ptr<float>(), dout.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
                             has & 1 ? slopes.data_ptr<float>() : nullptr, has & 4 ? doc.data_ptr<int>() : nullptr,
                             has & 2 ? prefix.data_ptr<int>() : nullptr, has & 4 ? table.data_ptr() : nullptr, st.data(),
                             (int)B, (int)H, (int)Hkv, (int)S, (int)D, (int)ctx->saved_data["window"].toInt(),
                             (float)ctx->saved_data["softcap"].toDouble(), dtype_code(q), ws.ptr, nbytes, at.stream),
           "otx_mask_attn_bwd");
-    return {dq, dk, dv, Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
+    return {dq, dk, dv, Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
   }
 };
 
@@ -601,7 +606,8 @@ Tensor attention(const Tensor& q, const Tensor& k, const Tensor& v, const std::o
 Tensor masked_attention(const Tensor& q, const Tensor& k, const Tensor& v, const std::optional<Tensor>& slopes,
                         const std::optional<Tensor>& doc, const std::optional<Tensor>& prefix, int64_t window,
                         double softcap) {
-  return MaskedAttention::apply(q, k, v, slopes, doc, prefix, window, softcap);
+  const bool grad = at::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad() || v.requires_grad());
+  return MaskedAttention::apply(q, k, v, slopes, doc, prefix, window, softcap, grad);
 }
 Tensor rotary_heads(const Tensor& x, const Tensor& cos, const Tensor& sin, const std::optional<Tensor>& positions,
                     int64_t layout) {

@@ -844,30 +844,33 @@ size_t otx_mask_attn_bwd_workspace_bytes(int B, int H, int Hkv, int S, int D, in
   return mask_dsum_bytes(B, H, S) + (otx::mask_attn_splits(B, H, Hkv, S, documents != 0) ? (size_t)B * H * S * D * 8 : 0);
 }
 
-int otx_mask_attn_fwd(const void* q, const void* k, const void* v, void* o, float* lse, const float* slopes,
+int otx_mask_attn_fwd(const void* q, const void* k, const void* v, void* o, void* o_low, float* lse, const float* slopes,
                       const int32_t* doc_ids, const int32_t* prefix, void* table, const long* strides, int B, int H,
                       int Hkv, int S, int D, int window, float softcap, int dtype, void* stream) {
   otx::MaskAttnArgs a = {};
   int rc = mask_args(&a, slopes, doc_ids, prefix, table, B, H, Hkv, S, D, window, softcap, dtype);
   if (rc) return rc;
   if (!strides || !lse) return fail(OTX_EINVAL, "null pointer argument");
+  if (!aligned16(o_low)) return fail(OTX_EINVAL, "o_low must be 16-byte aligned");
   if ((rc = mask_strides("q", q, strides, dtype, a.sq)) || (rc = mask_strides("k", k, strides + 3, dtype, a.sk)) ||
       (rc = mask_strides("v", v, strides + 6, dtype, a.sv)) || (rc = mask_strides("o", o, strides + 9, dtype, a.so)))
     return rc;
   a.q = q, a.k = k, a.v = v, a.out = o, a.lse = lse;
+  a.low = dtype == OTX_DTYPE_BF16 ? (signed char*)o_low : nullptr;
   hipError_t e = doc_ids ? otx::launch_mask_table(doc_ids, table, B, S, (hipStream_t)stream) : hipSuccess;
   if (e == hipSuccess) e = otx::launch_mask_attn(dtype, D, false, a, (hipStream_t)stream);
   return e == hipSuccess ? OTX_OK : fail(OTX_EHIP, "masked attention launch failed: %s", hipGetErrorString(e));
 }
 
-int otx_mask_attn_bwd(const void* q, const void* k, const void* v, const void* o, const float* lse, const void* dout,
-                      void* dq, void* dk, void* dv, const float* slopes, const int32_t* doc_ids, const int32_t* prefix,
+int otx_mask_attn_bwd(const void* q, const void* k, const void* v, const void* o, const void* o_low, const float* lse,
+                      const void* dout, void* dq, void* dk, void* dv, const float* slopes, const int32_t* doc_ids, const int32_t* prefix,
                       const void* table, const long* strides, int B, int H, int Hkv, int S, int D, int window,
                       float softcap, int dtype, void* workspace, size_t workspace_bytes, void* stream) {
   otx::MaskAttnArgs a = {};
   int rc = mask_args(&a, slopes, doc_ids, prefix, (void*)table, B, H, Hkv, S, D, window, softcap, dtype);
   if (rc) return rc;
   if (!strides || !lse || !workspace) return fail(OTX_EINVAL, "null pointer argument");
+  if (!aligned16(o_low)) return fail(OTX_EINVAL, "o_low must be 16-byte aligned");
   if ((rc = mask_strides("q", q, strides, dtype, a.sq)) || (rc = mask_strides("k", k, strides + 3, dtype, a.sk)) ||
       (rc = mask_strides("v", v, strides + 6, dtype, a.sv)) || (rc = mask_strides("o", o, strides + 9, dtype, a.so)) ||
       (rc = mask_strides("dout", dout, strides + 12, dtype, a.sdo)) ||
@@ -881,6 +884,7 @@ int otx_mask_attn_bwd(const void* q, const void* k, const void* v, const void* o
     return fail(OTX_EINVAL, "workspace too small: %zu bytes given, %zu needed", workspace_bytes, need);
   a.q = q, a.k = k, a.v = v, a.o = o, a.lse = (float*)lse, a.dout = dout, a.dq = dq, a.dk = dk, a.dv = dv;
   a.dsum = (float*)workspace;
+  a.low = dtype == OTX_DTYPE_BF16 ? (signed char*)o_low : nullptr;
   if (otx::mask_attn_splits(B, H, Hkv, S, doc_ids != nullptr)) a.part = (float*)((char*)workspace + mask_dsum_bytes(B, H, S));
   hipError_t e = otx::launch_mask_attn(dtype, D, true, a, (hipStream_t)stream);
   return e == hipSuccess ? OTX_OK : fail(OTX_EHIP, "masked attention backward launch failed: %s", hipGetErrorString(e));
