@@ -272,7 +272,7 @@ int otx_swap_heads(const void* x, void* y, int B, int X, int Y, int D, int dtype
 
 /* Masked attention: document and prefix masks, padding, windows of any size,
  * tanh-capped scores, a linear distance bias, any sequence length up to 2^24.
- *   t_ij = softcap tanh(q_i.k_j / sqrt(D) / softcap)   (softcap 0: q_i.k_j / sqrt(D))
+ *   t_ij = softcap tanh(q_i.k_j / sqrt(D) / softcap)   (softcap 0: q_i.k_j / sqrt(D); otherwise 2^-20 .. 2^13)
  *   u_ij = t_ij - slopes[h] |i - j|                     (slopes NULL: t_ij)
  *   o_i  = sum_j softmax(u_i)_j v_j over the visible j; a row that sees nothing is 0
  *   j is visible to i when doc_ids[b][i] == doc_ids[b][j] >= 0 (doc_ids NULL: always) and

@@ -821,7 +821,8 @@ static int mask_args(otx::MaskAttnArgs* a, const float* slopes, const int32_t* d
   if (rc) return rc;
   if (dtype != OTX_DTYPE_F32 && dtype != OTX_DTYPE_BF16) return fail(OTX_EINVAL, "dtype code %d not supported", dtype);
   if (window < 0) return fail(OTX_EINVAL, "window %d must not be negative", window);
-  if (!(softcap >= 0.0f && softcap <= 3e38f)) return fail(OTX_EINVAL, "softcap %g must be 0 or positive", (double)softcap);
+  if (softcap != 0.0f && !(softcap >= 0x1p-20f && softcap <= 0x1p13f))
+    return fail(OTX_EINVAL, "softcap %g must be 0 or in [2^-20, 2^13]", (double)softcap);
   if (doc_ids && (!table || !aligned16(table))) return fail(OTX_EINVAL, "doc_ids need a 16-byte aligned block table");
   a->slopes = slopes, a->doc = doc_ids, a->prefix = prefix, a->table = table;
   a->B = B, a->H = H, a->Hkv = Hkv, a->S = S;
@@ -928,6 +929,7 @@ int otx_layer_norm_fwd(const void* x, const void* w, const void* b, void* y, flo
                        float eps, int dtype, void* stream) {
   int rc = check_layer_norm(rows, D, dtype);
   if (rc) return rc;
+  if (!(eps >= 0.0f)) return fail(OTX_EINVAL, "layer norm: eps %g must not be negative", (double)eps);
   if (!x || !w || !y || !mean || !rstd) return fail(OTX_EINVAL, "null pointer argument");
   hipError_t e = otx::launch_layer_norm_fwd(dtype, x, w, b, y, mean, rstd, rows, D, eps, (hipStream_t)stream);
   return e == hipSuccess ? OTX_OK : fail(OTX_EHIP, "layer norm launch failed: %s", hipGetErrorString(e));

@@ -126,8 +126,8 @@ def merge_heads(o: torch.Tensor) -> torch.Tensor:
 
 
 def layer_norm(x: torch.Tensor, w: torch.Tensor, b: torch.Tensor | None = None, eps: float = 1e-5) -> torch.Tensor:
-    """Layer norm over the last dimension, of any width: (x - mean) / sqrt(var + eps) * w + b, in x's dtype.
-    The gradients of w and b come back in their dtype."""
+    """Layer norm over the last dimension, of any width: (x - mean) / sqrt(var + eps) * w + b, in x's dtype, w and b
+    rounded to it.  The gradients of w and b come back in their dtype."""
     _need_gpu(x, w, *(() if b is None else (b,)))
     if x.dtype not in _DT:
         raise ValueError(f"dtype {x.dtype} not supported")

@@ -10,8 +10,6 @@ several times faster and not under that contract; its results repeat bit for bit
 
 from __future__ import annotations
 
-import math
-
 import torch
 
 from . import _nodes
@@ -19,6 +17,7 @@ from . import _nodes
 __all__ = ["masked_flash_attention", "document_positions"]
 
 _DTYPES = (torch.bfloat16, torch.float32)
+_CAPS = (2.0**-20, 2.0**13)  # a cap's scores err by about 2^-22 of it: 2^-9, half a step of bf16, at the greatest
 
 
 def _check_mask(name: str, t: torch.Tensor | None, shape: tuple[int, ...], dtype: torch.dtype,
@@ -47,7 +46,7 @@ def masked_flash_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, wi
 
     ``doc_ids`` int32 [B, S] (None: one document per row; negative: padding), ``prefix`` int32 [B] (None: 0),
     ``window`` in keys, the query's own included (0: all).  Scores are q.k / sqrt(D), capped to
-    softcap * tanh(score / softcap) where ``softcap`` is not 0, less slopes[h] * |i - j| where ``slopes``
+    softcap * tanh(score / softcap) where ``softcap`` (2^-20 .. 2^13) is not 0, less slopes[h] * |i - j| where ``slopes``
     (float32 [H], constants) are given.  A query that sees nothing, as one of padding, gets zeros, and its
     gradients are zero; what lies in rows that a query does not see, NaN included, does not reach it.
 
@@ -80,8 +79,8 @@ def masked_flash_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, wi
     if not isinstance(window, int) or isinstance(window, bool) or not 0 <= window < 1 << 31:
         raise ValueError(f"window must be 0 (all keys) or a positive number of keys, got {window!r}")
     softcap = float(softcap)
-    if not 0.0 <= softcap < math.inf:
-        raise ValueError(f"softcap must be 0 (none) or positive, got {softcap}")
+    if softcap != 0.0 and not _CAPS[0] <= softcap <= _CAPS[1]:
+        raise ValueError(f"softcap must be 0 (none) or in [{_CAPS[0]}, {_CAPS[1]}], got {softcap}")
     slopes = _check_mask("slopes", slopes, (H,), torch.float32, q.device)
     doc_ids = _check_mask("doc_ids", doc_ids, (B, S), torch.int32, q.device)
     prefix = _check_mask("prefix", prefix, (B,), torch.int32, q.device)

@@ -132,6 +132,10 @@ def scaled_rope_tables(seq_len: int, rotary_dim: int, theta: float, factor: floa
         raise ValueError(f"tables of {seq_len} positions and {rotary_dim} rotated columns")
     if not factor >= 1.0 or not np.isfinite(factor):
         raise ValueError(f"factor {factor} must be at least 1")
+    if not 1.0 < theta < np.inf:
+        raise ValueError(f"theta {theta} must exceed 1")
+    if attention_factor is not None and not 0.0 < attention_factor < np.inf:
+        raise ValueError(f"attention_factor {attention_factor} must be positive")
     freq = theta ** (-np.arange(0, rotary_dim, 2, dtype=np.float64) / rotary_dim)
     scale = 1.0
     if method == "linear":
