@@ -484,10 +484,15 @@ __device__ __forceinline__ void load_own(u32x4 (&f)[D * sizeof(T) / 32], const T
     f[ks] = *(const u32x4*)(base + (long)row * stride + (2 * ks + (lane >> 5)) * (16 / (int)sizeof(T)));
 }
 
-// The eight bits of x after those that its bf16 rounding keeps, signed.
+// The eight bits of x after those that its bf16 rounding keeps, signed, in bits 8 to 15.
 __device__ __forceinline__ int low_bits(float x) {
-  const uint32_t high = (uint32_t)Elem<uint16_t>::put(x) << 16;
-  return min((int)(__float_as_uint(x) - high) >> 8, 127);
+  const uint32_t high = (uint32_t)__builtin_bit_cast(uint16_t, (__bf16)x) << 16;
+  return min((int)(__float_as_uint(x) - high), 0x7fff);
+}
+__device__ __forceinline__ uint32_t low_bytes(float a, float b, float c, float d) {
+  const uint32_t ab = __builtin_amdgcn_perm(low_bits(b), low_bits(a), 0x0c0c0501);
+  const uint32_t cd = __builtin_amdgcn_perm(low_bits(d), low_bits(c), 0x05010c0c);
+  return ab | cd;
 }
 __device__ __forceinline__ float with_low(float high, int low) { return __uint_as_float(__float_as_uint(high) + ((uint32_t)low << 8)); }
 
@@ -530,10 +535,8 @@ __device__ __forceinline__ void store_rows(O* out, long stride, int row0, int S,
     for (int dt = 0; dt < D / 32; dt++)
 #pragma unroll
       for (int g = 0; g < 4; g++) {
-        uint32_t w = 0;
-#pragma unroll
-        for (int i = 0; i < 4; i++) w |= (uint32_t)(low_bits(acc[dt][4 * g + i] * f) & 255) << (8 * i);
-        *(uint32_t*)(lds + n * D + (((2 * dt + g / 2) ^ (n & (CL - 1))) << 4) + 8 * (g & 1) + 4 * h) = w;
+        *(uint32_t*)(lds + n * D + (((2 * dt + g / 2) ^ (n & (CL - 1))) << 4) + 8 * (g & 1) + 4 * h) =
+            low_bytes(acc[dt][4 * g] * f, acc[dt][4 * g + 1] * f, acc[dt][4 * g + 2] * f, acc[dt][4 * g + 3] * f);
       }
 #pragma unroll
     for (int i = 0; i < CL / 2; i++) {
@@ -577,12 +580,7 @@ __device__ __forceinline__ void join_rows(O* out, long stride, int row0, int S, 
 #pragma unroll
         for (int e = 0; e < 4; e++) v[e] = (__bf16)o[e];
         *(bf16x4*)to = v;
-        if (low) {
-          uint32_t l = 0;
-#pragma unroll
-          for (int e = 0; e < 4; e++) l |= (uint32_t)(low_bits(o[e]) & 255) << (8 * e);
-          *(uint32_t*)(low + (long)(row0 + r) * D + c * 4) = l;
-        }
+        if (low) *(uint32_t*)(low + (long)(row0 + r) * D + c * 4) = low_bytes(o[0], o[1], o[2], o[3]);
       } else {
         *(f32x4*)to = o;
       }
@@ -615,24 +613,34 @@ __global__ void __launch_bounds__(256) mask_table_kernel(const int* doc, i32x4* 
 }
 
 // ---- backward: the weight and its gradient of one pair ------------------------------------------------
-// Element r of sv holds the raw dot product q.k, of dpv the product dO.v; on return p and dS (without sigma).
-template <typename T, bool PLAIN>
-__device__ __forceinline__ void weight(const MaskAttnArgs& a, f32x16& sv, f32x16& dpv, int r, float slope, float cs,
-                                       float lse, float dsum, int delta) {
-  const float s = sv[r], dp = dpv[r];
-  float u = s * cs, g = 1.0f;
-  if constexpr (PLAIN) {
-    sv[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s, cs, -lse));
+// What a score goes through: nothing; the distance bias; the cap (and the bias, of slope 0 where none is
+// given: two of some twenty instructions a pair).  Of the kernel's type, so that no pair has a branch.
+enum { kPlain, kBiased, kCapped };
+
+struct Score {
+  float cs, soc, cl, slope;  // sigma log2 e, sigma / cap, cap log2 e, slope log2 e
+  __device__ __forceinline__ Score(const MaskAttnArgs& a, int head)
+      : cs(a.sigma * kLog2e), soc(a.sigma / a.cap), cl(a.cap * kLog2e), slope(a.slopes ? a.slopes[head] * kLog2e : 0.0f) {}
+};
+
+// Element r of sv holds the raw dot product q.k, of dpv the product dO.v; on return p and dS (without
+// sigma).  distance: i - j, exact up to 2^24.
+template <typename T, int KIND>
+__device__ __forceinline__ void weight(const Score& c, f32x16& sv, f32x16& dpv, int r, float lse, float dsum,
+                                       float distance) {
+  const float s = sv[r];
+  float u, g = 1.0f;
+  if constexpr (KIND == kCapped) {
+    const float t = cap_tanh<T>(s, c.soc);
+    u = __builtin_fmaf(t, c.cl, -lse);
+    g = __builtin_fmaf(-t, t, 1.0f);
   } else {
-    if (a.cap > 0.0f) {
-      const float t = cap_tanh<T>(s, a.sigma / a.cap);
-      u = a.cap * kLog2e * t;
-      g = __builtin_fmaf(-t, t, 1.0f);
-    }
-    if (a.slopes) u = __builtin_fmaf(-slope, fabsf((float)delta), u);
-    sv[r] = __builtin_amdgcn_exp2f(u - lse);
+    u = __builtin_fmaf(s, c.cs, -lse);
   }
-  dpv[r] = sv[r] * (dp - dsum) * g;
+  if constexpr (KIND != kPlain) u = __builtin_fmaf(-c.slope, fabsf(distance), u);
+  sv[r] = __builtin_amdgcn_exp2f(u);
+  dpv[r] = sv[r] * (dpv[r] - dsum);
+  if constexpr (KIND == kCapped) dpv[r] *= g;
 }
 
 // ---- rows next to non-finite values ------------------------------------------------------------------
@@ -727,7 +735,7 @@ __device__ __forceinline__ void careful_row(const MaskAttnArgs& a, int b, int he
     if constexpr (WHAT == kForward) {
       const float o = l == 0.0f ? 0.0f : x[c] / l;
       ((T*)a.out)[b * a.so[0] + head * a.so[1] + own * a.so[2] + d] = Elem<T>::put(o);
-      if (a.low) a.low[row * D + d] = (signed char)low_bits(o);
+      if (a.low) a.low[row * D + d] = (signed char)(low_bits(o) >> 8);
     } else if constexpr (WHAT == kDQ) {
       ((T*)a.dq)[b * a.sdq[0] + head * a.sdq[1] + own * a.sdq[2] + d] = Elem<T>::put(x[c] * a.sigma);
     } else if constexpr (WHAT == kDKDVPart) {
@@ -751,7 +759,7 @@ __device__ __forceinline__ bool met_nonfinite(const Largest<T>& largest, int& lb
 
 // ---- forward -------------------------------------------------------------------------------------
 // Tiles are copied one ahead into the other of two buffers, with one barrier a tile.
-template <typename T, int D, bool PLAIN, bool TEAM>
+template <typename T, int D, int KIND, bool TEAM>
 __global__ void __launch_bounds__(kThreads, TEAM || sizeof(T) * D == 512 ? 1 : 2) mask_attn_fwd_kernel(const MaskAttnArgs a) {
   using L = Tile<T, D>;
   constexpr int BN = TEAM ? 32 : tile_rows<T>(), NT = BN / 32, BM = TEAM ? 32 : 128, BYTES = BN * L::RB;
@@ -765,7 +773,6 @@ __global__ void __launch_bounds__(kThreads, TEAM || sizeof(T) * D == 512 ? 1 : 2
   char (*lk_)[BYTES] = (char (*)[BYTES])tiles + set * 2 * NB, (*lv_)[BYTES] = lk_ + NB;
   const int S = a.S, nq = (S + BM - 1) / BM, nk = (S + BN - 1) / BN, nb = (S + kTab - 1) / kTab;
   const long total = (long)a.B * a.H * nq;
-  const float cs = a.sigma * kLog2e;
   const uint32_t row_k = L::row_base(lds_address(lk_), lane), col_v = L::col_base(lds_address(lv_), lane);
   if (threadIdx.x == 0) lbad = -1;
   int seq = 0;  // items so far: lbad names the last one that met a non-finite value
@@ -777,7 +784,7 @@ __global__ void __launch_bounds__(kThreads, TEAM || sizeof(T) * D == 512 ? 1 : 2
     const int* doc = a.doc ? a.doc + (long)b * S : nullptr;
     const i32x4* table = a.doc ? (const i32x4*)a.table + (long)b * nb : nullptr;
     const Band band = {S, a.window, a.prefix ? min(max(a.prefix[b], 0), S) : 0};
-    const float slope = !PLAIN && a.slopes ? a.slopes[hq] * kLog2e : 0.0f;
+    const Score sc(a, hq);
     Stage<T, D, BN, TEAM> gk, gv;
     gk.init((const T*)a.k + b * a.sk[0] + hk * a.sk[1], a.sk[2]);
     gv.init((const T*)a.v + b * a.sv[0] + hk * a.sv[1], a.sv[2]);
@@ -832,25 +839,18 @@ __global__ void __launch_bounds__(kThreads, TEAM || sizeof(T) * D == 512 ? 1 : 2
               read_step(vc, av, ks);
             fence_schedule();
           }
-        if constexpr (!PLAIN) {  // to scores in units of log 2
-          if (a.cap > 0.0f) {
-            const float soc = a.sigma / a.cap, cl = a.cap * kLog2e;
+        if constexpr (KIND != kPlain) {  // to scores in units of log 2
 #pragma unroll
-            for (int t = 0; t < NT; t++)
+          for (int t = 0; t < NT; t++)
 #pragma unroll
-              for (int r = 0; r < 16; r++) s[t][r] = cl * cap_tanh<T>(s[t][r], soc);
-          } else {
-#pragma unroll
-            for (int t = 0; t < NT; t++)
-#pragma unroll
-              for (int r = 0; r < 16; r++) s[t][r] *= cs;
-          }
-          if (a.slopes) {
+            for (int r = 0; r < 16; r++) s[t][r] = KIND == kCapped ? sc.cl * cap_tanh<T>(s[t][r], sc.soc) : sc.cs * s[t][r];
+          if (KIND == kBiased || a.slopes) {
+            const float d0 = (float)(qi - k0 - 4 * h);
 #pragma unroll
             for (int t = 0; t < NT; t++)
 #pragma unroll
               for (int r = 0; r < 16; r++)
-                s[t][r] = __builtin_fmaf(-slope, fabsf((float)(qi - (k0 + 32 * t + otx_row(r, 0) + 4 * h))), s[t][r]);
+                s[t][r] = __builtin_fmaf(-sc.slope, fabsf(d0 - (float)(32 * t + otx_row(r, 0))), s[t][r]);
           }
         }
         if (rare(cut)) {
@@ -865,7 +865,7 @@ __global__ void __launch_bounds__(kThreads, TEAM || sizeof(T) * D == 512 ? 1 : 2
 #pragma unroll
           for (int r = 0; r < 16; r++) top = fmaxf(top, s[t][r]);
         top = max_halves(top);
-        if constexpr (PLAIN) top *= cs;
+        if constexpr (KIND == kPlain) top *= sc.cs;
         // The statistics move only where a maximum grows by more than 2^8: weights stay below 2^8 and
         // the sums, in binary32, lose nothing; most tiles then leave the accumulator as it is.
         if (__ballot(top > m + 8.0f)) {
@@ -882,7 +882,7 @@ __global__ void __launch_bounds__(kThreads, TEAM || sizeof(T) * D == 512 ? 1 : 2
         for (int t = 0; t < NT; t++) {
 #pragma unroll
           for (int r = 0; r < 16; r++) {
-            s[t][r] = __builtin_amdgcn_exp2f(PLAIN ? __builtin_fmaf(s[t][r], cs, -mu) : s[t][r] - mu);
+            s[t][r] = __builtin_amdgcn_exp2f(KIND == kPlain ? __builtin_fmaf(s[t][r], sc.cs, -mu) : s[t][r] - mu);
             l += s[t][r];
           }
         }
@@ -943,7 +943,7 @@ __global__ void __launch_bounds__(kThreads, TEAM || sizeof(T) * D == 512 ? 1 : 2
 }
 
 // ---- backward: dQ, and D_i on the way ---------------------------------------------------------------
-template <typename T, int D, bool PLAIN, bool TEAM>
+template <typename T, int D, int KIND, bool TEAM>
 __global__ void __launch_bounds__(kThreads, sizeof(T) == 2 && !TEAM ? 2 : 1) mask_attn_dq_kernel(const MaskAttnArgs a) {
   using L = Tile<T, D>;
   constexpr int BN = TEAM ? 32 : tile_rows<T>(), NT = BN / 32, BM = TEAM ? 32 : 128, BYTES = BN * L::RB;
@@ -956,7 +956,6 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 2 && !TEAM ? 2 : 1) mas
   char (*lk_)[BYTES] = (char (*)[BYTES])tiles + set * 2 * NB, (*lv_)[BYTES] = lk_ + NB;
   const int S = a.S, nq = (S + BM - 1) / BM, nk = (S + BN - 1) / BN, nb = (S + kTab - 1) / kTab;
   const long total = (long)a.B * a.H * nq;
-  const float cs = a.sigma * kLog2e;
   const uint32_t row_k = L::row_base(lds_address(lk_), lane), col_k = L::col_base(lds_address(lk_), lane);
   const uint32_t row_v = L::row_base(lds_address(lv_), lane);
   if (threadIdx.x == 0) lbad = -1;
@@ -969,7 +968,7 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 2 && !TEAM ? 2 : 1) mas
     const int* doc = a.doc ? a.doc + (long)b * S : nullptr;
     const i32x4* table = a.doc ? (const i32x4*)a.table + (long)b * nb : nullptr;
     const Band band = {S, a.window, a.prefix ? min(max(a.prefix[b], 0), S) : 0};
-    const float slope = !PLAIN && a.slopes ? a.slopes[hq] * kLog2e : 0.0f;
+    const Score sc(a, hq);
     Stage<T, D, BN, TEAM> gk, gv;
     gk.init((const T*)a.k + b * a.sk[0] + hk * a.sk[1], a.sk[2]);
     gv.init((const T*)a.v + b * a.sv[0] + hk * a.sv[1], a.sv[2]);
@@ -1026,6 +1025,7 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 2 && !TEAM ? 2 : 1) mas
         const int* lid = lids[set][buf];
         if constexpr (TEAM) arrived_here(); else arrived();
         if (NB == 2) advance();
+        const float d0 = (float)(qi - k0 - 4 * h);
         if (rare(cut)) gk.look(lk, largest);
 #pragma unroll
         for (int t = 0; t < NT; t++) {
@@ -1048,7 +1048,7 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 2 && !TEAM ? 2 : 1) mas
           fence_schedule();
 #pragma unroll
           for (int r = 0; r < 16; r++)
-            weight<T, PLAIN>(a, s, dp, r, slope, cs, lse, dsum, qi - (k0 + 32 * t + 4 * h + otx_row(r, 0)));
+            weight<T, KIND>(sc, s, dp, r, lse, dsum, d0 - (float)(32 * t + otx_row(r, 0)));
           if (rare(cut)) {
             mask_block<true>(band, ids, lid + 32 * t, k0 + 32 * t, qi, qid >= 0, qid, h,
                              [&](int r, bool drop) { dp[r] = drop ? 0.0f : dp[r]; });
@@ -1078,7 +1078,7 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 2 && !TEAM ? 2 : 1) mas
 // ---- backward: dK and dV ----------------------------------------------------------------------------
 // SPLIT: a workgroup takes one query head and writes binary32 sums to a.part, which
 // mask_attn_join_kernel adds over the group; otherwise it takes the group's heads one after the other.
-template <typename T, int D, bool PLAIN, bool SPLIT, bool TEAM>
+template <typename T, int D, int KIND, bool SPLIT, bool TEAM>
 __global__ void __launch_bounds__(kThreads, sizeof(T) * D == 128 && !TEAM ? 2 : 1) mask_attn_dkdv_kernel(const MaskAttnArgs a) {
   using L = Tile<T, D>;
   constexpr int BN = TEAM ? 32 : tile_rows<T>(), NT = BN / 32, BM = TEAM ? 32 : 128, BYTES = BN * L::RB;
@@ -1094,7 +1094,6 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) * D == 128 && !TEAM ? 2 : 
   const int S = a.S, nkb = (S + BM - 1) / BM, nq = (S + BN - 1) / BN, nb = (S + kTab - 1) / kTab;
   const int group = a.H / a.Hkv, heads = SPLIT ? a.H : a.Hkv;
   const long total = (long)a.B * heads * nkb;
-  const float cs = a.sigma * kLog2e;
   const uint32_t row_q = L::row_base(lds_address(lq_), lane), col_q = L::col_base(lds_address(lq_), lane);
   const uint32_t row_g = L::row_base(lds_address(lg_), lane), col_g = L::col_base(lds_address(lg_), lane);
   if (threadIdx.x == 0) lbad = -1;
@@ -1163,7 +1162,8 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) * D == 128 && !TEAM ? 2 : 
         const int q0 = qb * BN, q1 = q0 + BN - 1;
         const bool cut = it.cut, ids = it.mixed;
         const int* lid = lids[set][buf];
-        const float slope = !PLAIN && a.slopes ? a.slopes[hq] * kLog2e : 0.0f;
+        const Score sc(a, hq);
+        const float d0 = (float)(q0 + 4 * h - kj);
         if constexpr (TEAM) arrived_here(); else arrived();
         if (NB == 2) advance();
         if (MASKED && rare(cut)) {
@@ -1186,8 +1186,7 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) * D == 128 && !TEAM ? 2 : 
           dp[t] = mma_rows<T>(gr.f[ks], vf[ks], dp[t]);
         };
         auto soft = [&](int t, int r) {
-          weight<T, PLAIN>(a, s[t], dp[t], r, slope, cs, x[r >> 2][r & 3], y[r >> 2][r & 3],
-                           q0 + 32 * t + 4 * h + otx_row(r, 0) - kj);
+          weight<T, KIND>(sc, s[t], dp[t], r, x[r >> 2][r & 3], y[r >> 2][r & 3], d0 + (float)(32 * t + otx_row(r, 0)));
         };
         const uint32_t rq = row_q + off, rg = row_g + off, cq = col_q + off, cg = col_g + off;
         qr.read(rq);
@@ -1350,48 +1349,47 @@ static bool team_of(int B, int heads, int S) {
   return S > 2 * tile_rows<T>() && blocks * (sizeof(T) == 2 ? 2 : 1) <= otx_cu_count();
 }
 
-template <typename T, int D, bool PLAIN>
+template <typename T, int D, int KIND>
 static hipError_t fwd_of(const MaskAttnArgs& a, hipStream_t st) {
   if (team_of<T>(a.B, a.H, a.S))
-    mask_attn_fwd_kernel<T, D, PLAIN, true><<<grid_of((long)a.B * a.H * ((a.S + 31) / 32)), kThreads, 0, st>>>(a);
+    mask_attn_fwd_kernel<T, D, KIND, true><<<grid_of((long)a.B * a.H * ((a.S + 31) / 32)), kThreads, 0, st>>>(a);
   else
-    mask_attn_fwd_kernel<T, D, PLAIN, false><<<grid_of((long)a.B * a.H * ((a.S + 127) / 128)), kThreads, 0, st>>>(a);
+    mask_attn_fwd_kernel<T, D, KIND, false><<<grid_of((long)a.B * a.H * ((a.S + 127) / 128)), kThreads, 0, st>>>(a);
   return hipGetLastError();
 }
 
-template <typename T, int D, bool PLAIN, bool SPLIT>
+template <typename T, int D, int KIND, bool SPLIT>
 static void dkdv_of(const MaskAttnArgs& a, int heads, hipStream_t st) {
   if (team_of<T>(a.B, heads, a.S))
-    mask_attn_dkdv_kernel<T, D, PLAIN, SPLIT, true><<<grid_of((long)a.B * heads * ((a.S + 31) / 32)), kThreads, 0, st>>>(a);
+    mask_attn_dkdv_kernel<T, D, KIND, SPLIT, true><<<grid_of((long)a.B * heads * ((a.S + 31) / 32)), kThreads, 0, st>>>(a);
   else
-    mask_attn_dkdv_kernel<T, D, PLAIN, SPLIT, false><<<grid_of((long)a.B * heads * ((a.S + 127) / 128)), kThreads, 0, st>>>(a);
+    mask_attn_dkdv_kernel<T, D, KIND, SPLIT, false><<<grid_of((long)a.B * heads * ((a.S + 127) / 128)), kThreads, 0, st>>>(a);
 }
 
-template <typename T, int D, bool PLAIN>
+template <typename T, int D, int KIND>
 static hipError_t bwd_of(const MaskAttnArgs& a, hipStream_t st) {
   if (team_of<T>(a.B, a.H, a.S))
-    mask_attn_dq_kernel<T, D, PLAIN, true><<<grid_of((long)a.B * a.H * ((a.S + 31) / 32)), kThreads, 0, st>>>(a);
+    mask_attn_dq_kernel<T, D, KIND, true><<<grid_of((long)a.B * a.H * ((a.S + 31) / 32)), kThreads, 0, st>>>(a);
   else
-    mask_attn_dq_kernel<T, D, PLAIN, false><<<grid_of((long)a.B * a.H * ((a.S + 127) / 128)), kThreads, 0, st>>>(a);
+    mask_attn_dq_kernel<T, D, KIND, false><<<grid_of((long)a.B * a.H * ((a.S + 127) / 128)), kThreads, 0, st>>>(a);
   if (a.part) {
-    dkdv_of<T, D, PLAIN, true>(a, a.H, st);
+    dkdv_of<T, D, KIND, true>(a, a.H, st);
     mask_attn_join_kernel<T, D><<<grid_of(((long)a.B * a.Hkv * a.S * (D / 2) + 255) / 256), 256, 0, st>>>(a);
   } else {
-    dkdv_of<T, D, PLAIN, false>(a, a.Hkv, st);
+    dkdv_of<T, D, KIND, false>(a, a.Hkv, st);
   }
   return hipGetLastError();
 }
 
 hipError_t launch_mask_attn(int dtype, int D, bool backward, const MaskAttnArgs& a, hipStream_t st) {
-  const bool plain = !(a.cap > 0.0f) && !a.slopes;
-#define OTX_MA(T, DD) \
-  return backward ? (plain ? bwd_of<T, DD, true>(a, st) : bwd_of<T, DD, false>(a, st)) \
-                  : (plain ? fwd_of<T, DD, true>(a, st) : fwd_of<T, DD, false>(a, st));
-  if (dtype == 1) {
-    if (D == 64) OTX_MA(uint16_t, 64) else OTX_MA(uint16_t, 128)
-  }
-  if (D == 64) OTX_MA(float, 64) else OTX_MA(float, 128)
+  const int kind = a.cap > 0.0f ? kCapped : a.slopes ? kBiased : kPlain;
+#define OTX_MA(T, DD, KIND) \
+  if (dtype == (sizeof(T) == 2) && D == DD && kind == KIND) return backward ? bwd_of<T, DD, KIND>(a, st) : fwd_of<T, DD, KIND>(a, st);
+#define OTX_MA3(T, DD) OTX_MA(T, DD, kPlain) OTX_MA(T, DD, kBiased) OTX_MA(T, DD, kCapped)
+  OTX_MA3(uint16_t, 64) OTX_MA3(uint16_t, 128) OTX_MA3(float, 64) OTX_MA3(float, 128)
+#undef OTX_MA3
 #undef OTX_MA
+  return hipErrorInvalidValue;
 }
 
 }  // namespace otx
