@@ -484,10 +484,10 @@ __device__ __forceinline__ void load_own(u32x4 (&f)[D * sizeof(T) / 32], const T
     f[ks] = *(const u32x4*)(base + (long)row * stride + (2 * ks + (lane >> 5)) * (16 / (int)sizeof(T)));
 }
 
-// The eight bits of x after those that its bf16 rounding keeps, signed, in bits 8 to 15.
+// The eight bits of x after those that its bf16 rounding keeps, signed and rounded, in bits 8 to 15.
 __device__ __forceinline__ int low_bits(float x) {
   const uint32_t high = (uint32_t)__builtin_bit_cast(uint16_t, (__bf16)x) << 16;
-  return min((int)(__float_as_uint(x) - high), 0x7fff);
+  return min((int)(__float_as_uint(x) + 128 - high), 0x7fff);
 }
 __device__ __forceinline__ uint32_t low_bytes(float a, float b, float c, float d) {
   const uint32_t ab = __builtin_amdgcn_perm(low_bits(b), low_bits(a), 0x0c0c0501);
@@ -882,7 +882,10 @@ __global__ void __launch_bounds__(kThreads, TEAM || sizeof(T) * D == 512 ? 1 : 2
         for (int t = 0; t < NT; t++) {
 #pragma unroll
           for (int r = 0; r < 16; r++) {
-            s[t][r] = __builtin_amdgcn_exp2f(KIND == kPlain ? __builtin_fmaf(s[t][r], sc.cs, -mu) : s[t][r] - mu);
+            // binary32: the maximum's own weight is 1 to the bit (bf16 rounds it to that)
+            const float u = KIND != kPlain ? s[t][r] - mu
+                            : sizeof(T) == 4 ? s[t][r] * sc.cs - mu : __builtin_fmaf(s[t][r], sc.cs, -mu);
+            s[t][r] = __builtin_amdgcn_exp2f(u);
             l += s[t][r];
           }
         }
@@ -990,21 +993,30 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 2 && !TEAM ? 2 : 1) mas
       load_own<T, D>(qf, (const T*)a.q + b * a.sq[0] + hq * a.sq[1], a.sq[2], qr, lane);
       load_own<T, D>(gf, (const T*)a.dout + b * a.sdo[0] + hq * a.sdo[1], a.sdo[2], qr, lane);
       const long row = ((long)b * a.H + hq) * S + qr;
+      // D_i by the matrix unit, in the order of dP's own products: where a row sees one key, O_i is its v
+      // and dP - D_i is 0.  The products of 32 rows with 32 rows hold it on the diagonal.
       float dsum = 0.0f;
       {
-        const T* op = (const T*)a.o + b * a.so[0] + hq * a.so[1] + qr * a.so[2];
+        u32x4 of[L::KS];
+        load_own<T, D>(of, (const T*)a.o + b * a.so[0] + hq * a.so[1], a.so[2], qr, lane);
+        f32x16 dd = {};
 #pragma unroll
-        for (int ks = 0; ks < L::KS; ks++) {
-          const u32x4 of = *(const u32x4*)(op + (2 * ks + h) * (16 / (int)sizeof(T)));
-          uint2 low = make_uint2(0, 0);
-          if (sizeof(T) == 2 && a.low) low = *(const uint2*)(a.low + row * D + (2 * ks + h) * 8);
+        for (int ks = 0; ks < L::KS; ks++) dd = mma_rows<T>(of[ks], gf[ks], dd);
+        if (sizeof(T) == 2 && a.low) {
 #pragma unroll
-          for (int e = 0; e < Elem<T>::VEC; e++) {
-            float x = element<T>(of, e);
-            if constexpr (sizeof(T) == 2) x = with_low(x, (int)((e < 4 ? low.x : low.y) << (24 - 8 * (e & 3))) >> 24);
-            dsum = __builtin_fmaf(element<T>(gf[ks], e), x, dsum);
+          for (int ks = 0; ks < L::KS; ks++) {
+            const uint2 low = *(const uint2*)(a.low + row * D + (2 * ks + h) * 8);
+            bf16x8 x;
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+              const float high = element<T>(of[ks], e % Elem<T>::VEC);
+              x[e] = (__bf16)(with_low(high, (int)((e < 4 ? low.x : low.y) << (24 - 8 * (e & 3))) >> 24) - high);
+            }
+            dd = mma_rows<T>(__builtin_bit_cast(u32x4, x), gf[ks], dd);
           }
         }
+#pragma unroll
+        for (int r = 0; r < 16; r++) dsum = otx_row(r, 0) + 4 * h == (lane & 31) ? dd[r] : dsum;
         dsum = sum_halves(dsum);
       }
       if (qi < S && h == 0 && (!TEAM || wave == 0)) a.dsum[row] = dsum;

@@ -427,3 +427,15 @@ def test_gradients_of_rows_that_see_few_keys(L, S, n):
     for (name, (value, _)), x in list(zip(reference(q, k, v, do, visible(S, 0, doc)).items(), got))[1:3]:
         off = (x[:1].double().cpu() - value).norm() / value.norm()
         assert off < 0.0030, (name, float(off))
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("cap,alibi", [(0.0, False), (30.0, False), (0.0, True)])
+@pytest.mark.parametrize("S,n,window", [(1, 1, 0), (1, 300, 0), (40, 2, 1), (200, 1, 1), (200, 80, 1)])
+def test_rows_that_see_one_key(S, n, window, cap, alibi, dtype):
+    """Their weight is 1 whatever the score, so o is v, and dq and dk are 0, to the bit."""
+    (q, k, v, do), _ = make(1, 4, 2, S, 128, dtype, scale=2.0)
+    slopes = torch.full((4,), 0.5) if alibi else None
+    o, dq, dk, _ = run(*[torch.cat([t] * n) for t in (q, k, v, do)], window=window, softcap=cap, slopes=slopes)
+    assert torch.equal(o[:1].cpu(), v.repeat_interleave(2, 1))
+    assert (dq == 0).all() and (dk == 0).all()
