@@ -3,9 +3,10 @@
 // one rounding to the storage type.  Pairs are (2 i, 2 i + 1) or (i, i + R / 2); columns R .. D - 1
 // are copied.  The gradient is the transpose, the same kernel with -s.
 //
-// Bound by memory: x is read once and written once, in the other order of heads and rows.  A thread
-// takes one unit of V pairs (two accesses of up to 16 bytes, at any address) of a row, and the same unit of several heads,
-// so that the position, c and s are read once for all of them.
+// Bound by memory: x is read once and written once, in the other order of heads and rows.  A thread takes
+// one unit of V pairs (two accesses of up to 16 bytes, at any address) of a row, and the same unit of several
+// heads, so that the position, c and s are read once for all of them.  4 x 4096 rows of 16 heads of 128 bf16
+// columns, pairs interleaved: 30 us for 134 MB and the tables, 4.5 TB/s (a large copy reaches 5.2).
 #include "otx_args.h"
 #include "otx_common.h"
 
