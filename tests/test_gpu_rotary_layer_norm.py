@@ -160,7 +160,8 @@ NORM = [
     (BF, (37, 2048), True), (F32, (9, 2052), True), (BF, (6, 2049), True), (F32, (5, 1000), True), (BF, (33, 128), True),
     (BF, (4, 8192), True), (F32, (3, 5005), False), (BF, (3, 8200), True), (F32, (2, 16384), True), (BF, (3, 12001), True),
     (F32, (2, 32768), True), (BF, (2, 40000), True), (F32, (3, 33333), True), (F32, (4111, 40), True), (BF, (2500, 520), False),
-    (F32, (700, 9000), True),
+    (F32, (700, 9000), True), (F32, (9001, 200), True), (BF, (3001, 255), True), (BF, (5000, 300), False), (F32, (40000, 16), True),
+    (F32, (1500, 4000), True), (BF, (20000, 72), True), (BF, (600, 8191), True),
 ]
 
 
