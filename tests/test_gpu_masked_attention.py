@@ -439,3 +439,23 @@ def test_rows_that_see_one_key(S, n, window, cap, alibi, dtype):
     o, dq, dk, _ = run(*[torch.cat([t] * n) for t in (q, k, v, do)], window=window, softcap=cap, slopes=slopes)
     assert torch.equal(o[:1].cpu(), v.repeat_interleave(2, 1))
     assert (dq == 0).all() and (dk == 0).all()
+
+
+@pytest.mark.parametrize("S", [70, 300])
+def test_recomputed_and_unpacked_activations(S):
+    """Under checkpointing and through saved-tensor hooks, the same bytes; without a gradient, the same output."""
+    from torch.utils.checkpoint import checkpoint
+
+    (q, k, v, do), gen = make(2, 4, 2, S, 64, BF)
+    kw = dict(doc_ids=docs_of("packed", 2, S, gen).to(DEV), slopes=torch.full((4,), 0.1, device=DEV), softcap=20.0)
+    want = run(q, k, v, do, **kw)
+    leaves = [t.to(DEV).requires_grad_() for t in (q, k, v)]
+    with torch.no_grad():
+        assert torch.equal(masked_flash_attention(*leaves, **kw), want[0])
+    o = checkpoint(lambda *t: masked_flash_attention(*t, **kw), *leaves, use_reentrant=False)
+    for a, b in zip((o, *torch.autograd.grad(o, leaves, do.to(DEV))), want):
+        assert torch.equal(a, b)
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t.cpu(), lambda t: t.to(DEV)):
+        o = masked_flash_attention(*leaves, **kw)
+    for a, b in zip(torch.autograd.grad(o, leaves, do.to(DEV)), want[1:]):
+        assert torch.equal(a, b)
