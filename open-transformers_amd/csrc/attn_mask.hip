@@ -677,7 +677,7 @@ __device__ __forceinline__ void careful_row(const MaskAttnArgs& a, int b, int he
   const T* k = (const T*)a.k + b * a.sk[0] + hk * a.sk[1];
   const T* v = (const T*)a.v + b * a.sv[0] + hk * a.sv[1];
   float m = -INFINITY, l = 0.0f, x[C] = {}, y[C] = {};  // sums: O; dQ; dK and dV
-  const int heads = KEYS ? a.H / a.Hkv / (WHAT == kDKDVPart ? a.parts : 1) : 1;
+  const int heads = WHAT == kDKDV ? a.H / a.Hkv : 1;
   for (int hq = head; hq < head + heads; hq++) {
     const T* q = (const T*)a.q + b * a.sq[0] + hq * a.sq[1];
     const T* g = (const T*)a.dout + b * a.sdo[0] + hq * a.sdo[1];
@@ -740,9 +740,8 @@ __device__ __forceinline__ void careful_row(const MaskAttnArgs& a, int b, int he
     } else if constexpr (WHAT == kDQ) {
       ((T*)a.dq)[b * a.sdq[0] + head * a.sdq[1] + own * a.sdq[2] + d] = Elem<T>::put(x[c] * a.sigma);
     } else if constexpr (WHAT == kDKDVPart) {
-      const long at = ((long)b * a.Hkv * a.parts + head / heads) * S + own;
-      a.part[at * D + d] = x[c] * a.sigma;
-      a.part[(at + (long)a.B * a.Hkv * a.parts * S) * D + d] = y[c];
+      a.part[row * D + d] = x[c] * a.sigma;
+      a.part[(row + (long)a.B * a.H * S) * D + d] = y[c];
     } else {
       ((T*)a.dk)[b * a.sdk[0] + hk * a.sdk[1] + own * a.sdk[2] + d] = Elem<T>::put(x[c] * a.sigma);
       ((T*)a.dv)[b * a.sdv[0] + hk * a.sdv[1] + own * a.sdv[2] + d] = Elem<T>::put(y[c]);
@@ -1098,12 +1097,12 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 2 && !TEAM ? 2 : 1) mas
 }
 
 // ---- backward: dK and dV ----------------------------------------------------------------------------
-// A workgroup takes a group's heads one after the other.  SPLIT: one of a.parts shares of them, and it writes
-// binary32 sums to a.part, which mask_attn_join_kernel adds.  A team takes one head.
+// SPLIT: a workgroup takes one query head and writes binary32 sums to a.part, which
+// mask_attn_join_kernel adds over the group; otherwise it takes the group's heads one after the other.
 // A wave holds its 32 keys' k, v, dK and dV, 384 registers at 128 columns, so one wave stays on a SIMD, and
 // the weights of one block of queries are formed beside the products of the other (below).  4 x 16 heads
-// over 4 x 4096 tokens 690 us, 795 TFLOP/s; packed in documents of 900, split in two, 353 us and 26 for the
-// join, 340 (the matrix pipe 0.25 busy, vector instructions 0.34, waits for LDS and barriers 0.29).  Measured and not
+// over 4 x 4096 tokens 690 us, 795 TFLOP/s; packed in documents of 900, split, 326 us and 49 for the join, 345
+// (the matrix pipe 0.25 busy, vector instructions 0.34, waits for LDS and barriers 0.29).  Measured and not
 // kept: four buffers in place of two (754 us against 704), the same interleaving for cut tiles (its masks
 // spill), workgroups that stay and take sorted blocks in turn (443 us against 420 on documents).
 template <typename T, int D, int KIND, bool SPLIT, bool TEAM>
@@ -1120,7 +1119,7 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) * D == 128 && !TEAM ? 2 : 
   const int set = TEAM ? wave : 0;
   char (*lq_)[BYTES] = (char (*)[BYTES])tiles + set * 2 * NB, (*lg_)[BYTES] = lq_ + NB;
   const int S = a.S, nkb = (S + BM - 1) / BM, nq = (S + BN - 1) / BN, nb = (S + kTab - 1) / kTab;
-  const int parts = SPLIT ? a.parts : 1, heads = a.Hkv * parts, share = a.H / heads;
+  const int group = a.H / a.Hkv, heads = SPLIT ? a.H : a.Hkv;
   const long total = (long)a.B * heads * nkb;
   const uint32_t row_q = L::row_base(lds_address(lq_), lane), col_q = L::col_base(lds_address(lq_), lane);
   const uint32_t row_g = L::row_base(lds_address(lg_), lane), col_g = L::col_base(lds_address(lg_), lane);
@@ -1129,14 +1128,14 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) * D == 128 && !TEAM ? 2 : 
 
   for (long w = blockIdx.x; w < total; w += gridDim.x) {
     // the first keys have the most queries, so they come first
-    const int bh = (int)(w % ((long)a.B * heads)), b = bh / heads, head = bh % heads, hk = head / parts;
+    const int bh = (int)(w % ((long)a.B * heads)), b = bh / heads, head = bh % heads, hk = SPLIT ? head / group : head;
     const int k0 = (int)(w / ((long)a.B * heads)) * BM, k1 = min(k0 + BM, S) - 1;
     const int kw0 = k0 + (TEAM ? 0 : 32 * wave), kw1 = min(kw0 + 31, S - 1), kj = kw0 + (lane & 31), kr = min(kj, S - 1);
     const int* doc = a.doc ? a.doc + (long)b * S : nullptr;
     const i32x4* table = a.doc ? (const i32x4*)a.table + (long)b * nb : nullptr;
     const Band band = {S, a.window, a.prefix ? min(max(a.prefix[b], 0), S) : 0};
     const Docs own = docs_of(table, k0 / kTab, k1 / kTab, nb);
-    const int first = head * share, last = first + share;
+    const int first = SPLIT ? head : hk * group, last = SPLIT ? first + 1 : first + group;
 
     auto item = [&]() {
       f32x16 dk[L::DT] = {}, dv[L::DT] = {};
@@ -1306,8 +1305,8 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) * D == 128 && !TEAM ? 2 : 
         }
       };
       if constexpr (SPLIT) {
-        float* p = a.part + ((long)b * heads + head) * S * D;
-        put(p, D, p + (long)a.B * heads * S * D, D);
+        float* p = a.part + ((long)b * a.H + first) * S * D;
+        put(p, D, p + (long)a.B * a.H * S * D, D);
       } else {
         put((T*)a.dk + b * a.sdk[0] + hk * a.sdk[1], a.sdk[2], (T*)a.dv + b * a.sdv[0] + hk * a.sdv[1], a.sdv[2]);
       }
@@ -1319,11 +1318,12 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) * D == 128 && !TEAM ? 2 : 
   }
 }
 
-// The sum of a group's partial dK and dV, heads ascending, four columns a thread.  Bound by memory: 4 x 4
-// groups x 4096 x 128 in two parts, 168 MB, 26 us, 6.4 TB/s (part of it from the last-level cache).
+// The sum of a group's partial dK and dV, heads ascending, four columns a thread.  Bound by memory: 4 x 16
+// heads x 4096 x 128, 302 MB, 49 us, 6.2 TB/s (part of it from the last-level cache).
 template <typename T, int D>
 __global__ void __launch_bounds__(256) mask_attn_join_kernel(const MaskAttnArgs a) {
-  const long n = (long)a.B * a.Hkv * a.S * (D / 4), half = (long)a.B * a.Hkv * a.parts * a.S * D;
+  const int group = a.H / a.Hkv;
+  const long n = (long)a.B * a.Hkv * a.S * (D / 4), half = (long)a.B * a.H * a.S * D;
   for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < 2 * n; i += (long)gridDim.x * 256) {
     const bool isv = i >= n;
     long e = isv ? i - n : i;
@@ -1332,9 +1332,9 @@ __global__ void __launch_bounds__(256) mask_attn_join_kernel(const MaskAttnArgs 
     const int s = (int)(e % a.S);
     e /= a.S;
     const int hk = (int)(e % a.Hkv), b = (int)(e / a.Hkv);
-    const float* p = a.part + (isv ? half : 0) + (((long)b * a.Hkv + hk) * a.parts * a.S + s) * D + d;
+    const float* p = a.part + (isv ? half : 0) + (((long)b * a.H + hk * group) * a.S + s) * D + d;
     float4 sum = *(const float4*)p;
-    for (int g = 1; g < a.parts; g++) {
+    for (int g = 1; g < group; g++) {
       const float4 x = *(const float4*)(p + (long)g * a.S * D);
       sum.x += x.x, sum.y += x.y, sum.z += x.z, sum.w += x.w;
     }
@@ -1348,18 +1348,14 @@ int grid_of(long work) { return (int)(work < (1 << 20) ? work : (1 << 20)); }
 
 }  // namespace
 
-// Over how many workgroups dK/dV splits a group of query heads: as few as make enough blocks to even out what
-// the compute units get, which takes more of them with long sequences (the first keys have the most
-// queries) and with documents (of unequal lengths).  It costs the partial sums.  Groups of four heads of 128
-// bf16 columns, whole and in four, in us: 128 blocks of 1024 tokens 232 and 79, 256 of 1024 152 and 156, 256
-// of 4096 563 and 374, 512 of 1024 201 and 327, of 4096 660 and 731; with documents of 500 tokens, 512
-// blocks, 541 and 385.  512 blocks, documents of 900: in four 333 and 48 for the join, in two 353 and 26.
-int mask_attn_parts(int B, int H, int Hkv, int S, bool documents) {
-  const long blocks = (long)B * Hkv * ((S + 127) / 128), enough = (documents ? 3 : S >= 2048 ? 2 : 1) * otx_cu_count();
-  const int group = H / Hkv;
-  int parts = 1;
-  while (parts < group && (blocks * parts < enough || group % parts)) parts++;
-  return parts;
+// Whether dK/dV splits a group of query heads over workgroups: that evens out what the compute units get,
+// which counts with few blocks, with long sequences (the first keys have the most queries) and with
+// documents (of unequal lengths), and costs the partial sums.  Groups of four heads of 128 bf16 columns,
+// whole and split, in us: 128 blocks of 1024 tokens 232 and 79, 256 of 1024 152 and 156, 256 of 4096 563
+// and 374, 512 of 1024 201 and 327, of 4096 660 and 731; with documents of 500 tokens 541 and 385.
+bool mask_attn_splits(int B, int H, int Hkv, int S, bool documents) {
+  const long blocks = (long)B * Hkv * ((S + 127) / 128);
+  return H > Hkv && blocks < (documents ? 3 : S >= 2048 ? 2 : 1) * otx_cu_count();
 }
 
 hipError_t launch_mask_table(const int* doc, void* table, int B, int S, hipStream_t st) {
@@ -1391,9 +1387,8 @@ static hipError_t fwd_of(const MaskAttnArgs& a, hipStream_t st) {
 }
 
 template <typename T, int D, int KIND, bool SPLIT>
-static void dkdv_of(const MaskAttnArgs& a, hipStream_t st) {
-  const int heads = a.Hkv * (SPLIT ? a.parts : 1);
-  if (heads == a.H && team_of<T>(a.B, heads, a.S))
+static void dkdv_of(const MaskAttnArgs& a, int heads, hipStream_t st) {
+  if (team_of<T>(a.B, heads, a.S))
     mask_attn_dkdv_kernel<T, D, KIND, SPLIT, true><<<grid_of((long)a.B * heads * ((a.S + 31) / 32)), kThreads, 0, st>>>(a);
   else
     mask_attn_dkdv_kernel<T, D, KIND, SPLIT, false><<<grid_of((long)a.B * heads * ((a.S + 127) / 128)), kThreads, 0, st>>>(a);
@@ -1406,10 +1401,10 @@ static hipError_t bwd_of(const MaskAttnArgs& a, hipStream_t st) {
   else
     mask_attn_dq_kernel<T, D, KIND, false><<<grid_of((long)a.B * a.H * ((a.S + 127) / 128)), kThreads, 0, st>>>(a);
   if (a.part) {
-    dkdv_of<T, D, KIND, true>(a, st);
+    dkdv_of<T, D, KIND, true>(a, a.H, st);
     mask_attn_join_kernel<T, D><<<grid_of(((long)a.B * a.Hkv * a.S * (D / 2) + 255) / 256), 256, 0, st>>>(a);
   } else {
-    dkdv_of<T, D, KIND, false>(a, st);
+    dkdv_of<T, D, KIND, false>(a, a.Hkv, st);
   }
   return hipGetLastError();
 }

@@ -47,7 +47,7 @@ hipError_t launch_swiglu(int dtype, int backward, const void* gu, const void* dh
 hipError_t launch_rope_heads(int dtype, int backward, const void* in, const float* cosv, const float* sinv, void* out,
                              int B, int Tn, int H, int D, hipStream_t st);
 hipError_t launch_swap_heads(int dtype, const void* in, void* out, int B, int X, int Y, int D, hipStream_t st);
-int mask_attn_parts(int B, int H, int Hkv, int S, bool documents);
+bool mask_attn_splits(int B, int H, int Hkv, int S, bool documents);
 hipError_t launch_mask_table(const int* doc, void* table, int B, int S, hipStream_t st);
 hipError_t launch_mask_attn(int dtype, int D, bool backward, const MaskAttnArgs& a, hipStream_t st);
 hipError_t launch_rotary(int dtype, const RotaryArgs& a, bool half, hipStream_t st);
@@ -842,8 +842,7 @@ static size_t mask_dsum_bytes(int B, int H, int S) { return ((size_t)B * H * S *
 
 size_t otx_mask_attn_bwd_workspace_bytes(int B, int H, int Hkv, int S, int D, int documents) {
   if (check_mask_shape(B, H, Hkv, S, D) != OTX_OK) return 0;
-  const int parts = otx::mask_attn_parts(B, H, Hkv, S, documents != 0);
-  return mask_dsum_bytes(B, H, S) + (parts > 1 ? (size_t)B * Hkv * parts * S * D * 8 : 0);
+  return mask_dsum_bytes(B, H, S) + (otx::mask_attn_splits(B, H, Hkv, S, documents != 0) ? (size_t)B * H * S * D * 8 : 0);
 }
 
 int otx_mask_attn_fwd(const void* q, const void* k, const void* v, void* o, void* o_low, float* lse, const float* slopes,
@@ -887,8 +886,7 @@ int otx_mask_attn_bwd(const void* q, const void* k, const void* v, const void* o
   a.q = q, a.k = k, a.v = v, a.o = o, a.lse = (float*)lse, a.dout = dout, a.dq = dq, a.dk = dk, a.dv = dv;
   a.dsum = (float*)workspace;
   a.low = dtype == OTX_DTYPE_BF16 ? (signed char*)o_low : nullptr;
-  a.parts = otx::mask_attn_parts(B, H, Hkv, S, doc_ids != nullptr);
-  if (a.parts > 1) a.part = (float*)((char*)workspace + mask_dsum_bytes(B, H, S));
+  if (otx::mask_attn_splits(B, H, Hkv, S, doc_ids != nullptr)) a.part = (float*)((char*)workspace + mask_dsum_bytes(B, H, S));
   hipError_t e = otx::launch_mask_attn(dtype, D, true, a, (hipStream_t)stream);
   return e == hipSuccess ? OTX_OK : fail(OTX_EHIP, "masked attention backward launch failed: %s", hipGetErrorString(e));
 }

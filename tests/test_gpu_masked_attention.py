@@ -459,20 +459,3 @@ def test_recomputed_and_unpacked_activations(S):
         o = masked_flash_attention(*leaves, **kw)
     for a, b in zip(torch.autograd.grad(o, leaves, do.to(DEV)), want[1:]):
         assert torch.equal(a, b)
-
-
-@pytest.mark.parametrize("dtype,D,bad", [(BF, 128, False), (BF, 64, True), (F32, 64, False)])
-def test_groups_split_in_fewer_parts_than_heads(dtype, D, bad):
-    """Documents, and blocks enough for two or three parts of a group of six heads; the first rows against binary64."""
-    B, H, Hkv, S = 140, 12, 2, 200
-    (q, k, v, do), gen = make(2, H, Hkv, S, D, dtype)
-    doc = docs_of("right", 2, S, gen)
-    if bad:  # in the padding: the rows beside it are done over one at a time
-        k[1, :, -1], v[1, :, -2], do[1, :, -1] = float("nan"), float("inf"), float("nan")
-    clean = [torch.nan_to_num(t, 0.0, 0.0, 0.0) for t in (q, k, v, do)]
-    want = reference(*clean, visible(S, 0, doc), storage=dtype)
-    for n in (B // 2, 3 * B // 8):
-        got = run(*[torch.cat([t] * n) for t in (q, k, v, do)], doc_ids=torch.cat([doc] * n))
-        compare([x[:2] for x in got], want)
-        for x in got:
-            assert torch.equal(x[-2:], x[:2])
