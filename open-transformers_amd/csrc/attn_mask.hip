@@ -1352,7 +1352,8 @@ int grid_of(long work) { return (int)(work < (1 << 20) ? work : (1 << 20)); }
 // which counts with few blocks, with long sequences (the first keys have the most queries) and with
 // documents (of unequal lengths), and costs the partial sums.  Groups of four heads of 128 bf16 columns,
 // whole and split, in us: 128 blocks of 1024 tokens 232 and 79, 256 of 1024 152 and 156, 256 of 4096 563
-// and 374, 512 of 1024 201 and 327, of 4096 660 and 731; with documents of 500 tokens 541 and 385.
+// and 374, 512 of 1024 201 and 327, of 4096 660 and 731; with documents of 500 tokens 541 and 385
+// (in two parts, half the sums: 4 x 4096 tokens in documents of 900, 688 us a pass where four take 665 to 680).
 bool mask_attn_splits(int B, int H, int Hkv, int S, bool documents) {
   const long blocks = (long)B * Hkv * ((S + 127) / 128);
   return H > Hkv && blocks < (documents ? 3 : S >= 2048 ? 2 : 1) * otx_cu_count();
